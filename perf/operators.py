@@ -303,7 +303,7 @@ def _plain_balance(st):
     counts.scatter_add_(0, (row.unsqueeze(1) * E + st.ids.long()).view(-1), torch.ones_like(st.ids).view(-1))
     counts = counts.view(B + 1, E)[:B]
     P = torch.zeros(B + 1, E, dtype=torch.float64, device=x.device).index_add_(0, row, p.double())[:B].float()
-    scale = (st.coef * E / topk) / (n * n).clamp_min(1) / (n > 0).float().sum().clamp_min(1)
+    scale = (st.coef * E / (topk * B)) / (n * n).clamp_min(1)          # a mean over the sequences given
     loss = (scale.unsqueeze(1) * counts.float() * P).sum()
     total = counts.sum(0, dtype=torch.int32)
     if st.grad == "none":
@@ -359,6 +359,6 @@ def exact(case, seed):
             counts = torch.bincount(st.ids[a:b][keep].long().view(-1), minlength=case["E"])
             total += counts
             parts.append(case["E"] / (case["topk"] * n) * (counts.double() * p[a:b][keep].mean(0)).sum())
-    loss = st.coef * torch.stack(parts).mean() if parts else x.sum() * 0
+    loss = st.coef / (len(cu) - 1) * torch.stack(parts).sum() if parts else x.sum() * 0
     out = (loss.detach(), None)
     return out if case["grad"] == "none" else out + (torch.autograd.grad(loss, x)[0],)
