@@ -334,6 +334,37 @@ int mlk_fused_experts_compute_static(const void* w1, const void* w2, const void*
                                      const int32_t* experts_map, int experts_map_len, const int32_t* tune,
                                      int32_t* status, int out_fp32, mlk_stream_t s);
 
+/* ---- 4-bit weights with group scales (no counterpart in the reference) ------------------------------------------- */
+
+/* W[m,k] = (q[m,k] - z[m,k/group]) * s[m,k/group]: q and z in 0..15, s in the activation type, group 32, 64 or 128, k whole
+ * groups, m a multiple of 16.  Laid out once at load time:
+ *   q  row-major nibbles [m, k/2] (low nibble = even k) -> [m/16][ceil(k/64)][32][16 bytes]   mlk_layoutA_w4
+ *   s, z  [m, k/group] -> [m/16][k/group][8][2], entry (r, h) = row r + 8 h of 16               mlk_layoutA_w4_groups
+ * Lane l = 4 r + t of a block holds four little-endian 32-bit words; word j has the nibble pair p (bits 4p and 16 + 4p) of row r + 8 (p & 1), k = 64 block + 16 j + 4 t + 2 (p >> 1) and the next k.
+ * Matrices stored back to back (the experts of a layer) are one matrix with all their rows. */
+
+/* inverse = 0: row-major src -> packed dst; inverse = 1: packed src -> row-major dst.  k % 32 == 0. */
+int mlk_layoutA_w4(const void* src, void* dst, int64_t m, int k, int inverse, mlk_stream_t s);
+/* elem_bytes: 2 (scales) or 1 (zero points). */
+int mlk_layoutA_w4_groups(const void* src, void* dst, int64_t m, int groups, int elem_bytes, mlk_stream_t s);
+/* C[n,m] = alpha * B[n,k] * W^T (+ bias), any n >= 0; dtype 0 / 1 = bf16 / fp16 scales, B, C and bias.  zeros may be NULL (8
+ * everywhere); of each zero point the low four bits count.  status: sticky error word of the bounded waits, or NULL. */
+int mlk_gemm_layoutA_w4(const void* A, const void* scales, const void* zeros, int group, const void* B, void* C, int m, int n,
+                        int k, int dtype, float alpha, const void* bias, int32_t* status, mlk_stream_t s);
+/* Expert compute with 4-bit weights: y[t] = sum_j topk_weights[t,j] * W2_e (silu(Wgate_e x_t) * (Wup_e x_t)), e =
+ * topk_ids[t,j] (through experts_map if given; ids without an expert here are skipped).  w1 [expert_count, 2 inter, hidden]
+ * (gate rows, then up rows) and w2 [expert_count, hidden, inter] packed, with their own group sizes; hidden and inter
+ * multiples of 32 and whole groups.  y [T, hidden] in the activation type, or fp32 un-rounded sums with out_fp32 != 0;
+ * every element of y is written.  workspace: mlk_experts_w4_workspace_bytes(...) bytes, 16-byte aligned, contents
+ * irrelevant, not shared by calls that can overlap on the GPU. */
+int64_t mlk_experts_w4_workspace_bytes(int batch_size, int expert_count, int topK, int hidden, int inter);
+int mlk_fused_experts_compute_w4(const void* w1, const void* w1_scales, const void* w1_zeros, int w1_group, const void* w2,
+                                 const void* w2_scales, const void* w2_zeros, int w2_group, const void* x, int batch_size,
+                                 int expert_count, int topK, int hidden, int inter, const int32_t* topk_ids,
+                                 const void* topk_weights, void* y, int dtype, int out_fp32, const int32_t* experts_map,
+                                 int experts_map_len, void* workspace, int64_t workspace_bytes, int32_t* status,
+                                 mlk_stream_t s);
+
 /* ---- expert-parallel token exchange (no counterpart in the reference, which is single-GPU) ------------------ */
 
 /* out[i,:] = x[idx[i],:] for n_rows rows of `hidden` 16-bit elements (hidden % 8 == 0); an index outside

@@ -64,6 +64,13 @@ PROTOTYPES = {
     "mlk_fused_experts_compute": (c_int, [c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int, c_vp, c_vp, c_vp,
                                           c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_vp,
                                           c_int, c_vp, c_i64, C.POINTER(C.c_int32), c_vp, c_int, c_vp]),
+    "mlk_layoutA_w4": (c_int, [c_vp, c_vp, c_i64, c_int, c_int, c_vp]),
+    "mlk_layoutA_w4_groups": (c_int, [c_vp, c_vp, c_i64, c_int, c_int, c_vp]),
+    "mlk_gemm_layoutA_w4": (c_int, [c_vp, c_vp, c_vp, c_int, c_vp, c_vp, c_int, c_int, c_int, c_int, c_f32, c_vp, c_vp, c_vp]),
+    "mlk_experts_w4_workspace_bytes": (c_i64, [c_int, c_int, c_int, c_int, c_int]),
+    "mlk_fused_experts_compute_w4": (c_int, [c_vp, c_vp, c_vp, c_int, c_vp, c_vp, c_vp, c_int, c_vp, c_int, c_int, c_int,
+                                             c_int, c_int, c_vp, c_vp, c_vp, c_int, c_int, c_vp, c_int, c_vp, c_i64, c_vp,
+                                             c_vp]),
     "mlk_ep_reduce_flag_bytes": (c_i64, []),
     "mlk_ep_reduce_recv_bytes": (c_i64, [c_int, c_i64, c_int]),
     "mlk_ep_reduce_shares": (c_int, [c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_i64, c_int, c_int, c_vp, c_vp]),

@@ -38,6 +38,10 @@ SOURCES = [
     "moe_decode.cu",
     "ep_reduce.cu",
     "moe_exchange.cu",
+    "w4_pack.cu",
+    "w4_dense.cu",
+    "w4_mma.cu",
+    "w4_experts.cu",
     "selector.cpp",
 ]
 

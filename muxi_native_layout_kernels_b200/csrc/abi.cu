@@ -9,6 +9,7 @@
 #include "moe.cuh"
 #include "selector.h"
 #include "status.h"
+#include "w4.cuh"
 
 namespace mlk {
 
@@ -186,6 +187,19 @@ int gemm_table(int table, int variant_x, int variant_c, const void* A, const flo
 }  // namespace mlk
 
 using namespace mlk;
+
+namespace {
+// No entry point is meant to throw; whatever does (an allocation of a launch cache) must not cross the C boundary.
+template <class F>
+int guarded(F&& f) {
+    clear_error();
+    try {
+        return f();
+    } catch (...) {
+        return fail(kCudaError, "out of host memory");
+    }
+}
+}  // namespace
 
 extern "C" {
 
@@ -514,6 +528,44 @@ int mlk_fused_experts_compute_static(const void* w1, const void* w2, const void*
                                    w2_scale, dtype, fp8_order, microBatchSize, experts_map, experts_map_len, tune, status,
                                    out_fp32);
     return launch_fused_experts_static(p, (cudaStream_t)s);
+}
+
+// ---- 4-bit weights ---------------------------------------------------------------------------------------------
+
+int mlk_layoutA_w4(const void* src, void* dst, int64_t m, int k, int inverse, mlk_stream_t s) {
+    return guarded([&] { return launch_w4_pack(src, dst, m, k, inverse, (cudaStream_t)s); });
+}
+
+int mlk_layoutA_w4_groups(const void* src, void* dst, int64_t m, int groups, int elem_bytes, mlk_stream_t s) {
+    return guarded([&] { return launch_w4_groups(src, dst, m, groups, elem_bytes, (cudaStream_t)s); });
+}
+
+int mlk_gemm_layoutA_w4(const void* A, const void* scales, const void* zeros, int group, const void* B, void* C, int m, int n,
+                        int k, int dtype, float alpha, const void* bias, int32_t* status, mlk_stream_t s) {
+    W4DenseParams p{};
+    p.w = W4Weights{reinterpret_cast<const uint8_t*>(A), scales, reinterpret_cast<const uint8_t*>(zeros), group};
+    p.X = B; p.C = C; p.bias = bias; p.alpha = alpha; p.m = m; p.n = n; p.k = k; p.dtype = dtype; p.status = status;
+    return guarded([&] { return launch_w4_dense(p, (cudaStream_t)s); });
+}
+
+int64_t mlk_experts_w4_workspace_bytes(int batch_size, int expert_count, int topK, int hidden, int inter) {
+    return w4_experts_workspace_bytes(batch_size, expert_count, topK, hidden, inter);
+}
+
+int mlk_fused_experts_compute_w4(const void* w1, const void* w1_scales, const void* w1_zeros, int w1_group, const void* w2,
+                                 const void* w2_scales, const void* w2_zeros, int w2_group, const void* x, int batch_size,
+                                 int expert_count, int topK, int hidden, int inter, const int32_t* topk_ids,
+                                 const void* topk_weights, void* y, int dtype, int out_fp32, const int32_t* experts_map,
+                                 int experts_map_len, void* workspace, int64_t workspace_bytes, int32_t* status,
+                                 mlk_stream_t s) {
+    W4ExpertsParams p{};
+    p.w1 = W4Weights{reinterpret_cast<const uint8_t*>(w1), w1_scales, reinterpret_cast<const uint8_t*>(w1_zeros), w1_group};
+    p.w2 = W4Weights{reinterpret_cast<const uint8_t*>(w2), w2_scales, reinterpret_cast<const uint8_t*>(w2_zeros), w2_group};
+    p.x = x; p.topk_ids = topk_ids; p.topk_weights = topk_weights; p.y = y;
+    p.T = batch_size; p.E = expert_count; p.topk = topK; p.H = hidden; p.I = inter; p.dtype = dtype; p.y_fp32 = out_fp32;
+    p.experts_map = experts_map; p.experts_map_len = experts_map_len;
+    p.workspace = workspace; p.workspace_bytes = workspace_bytes; p.status = status;
+    return guarded([&] { return launch_w4_experts(p, (cudaStream_t)s); });
 }
 
 }  // extern "C"

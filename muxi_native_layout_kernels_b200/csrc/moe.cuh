@@ -63,6 +63,9 @@ struct MoeParams {
 };
 
 int launch_fused_experts(const MoeParams& p, cudaStream_t s);
+// The fixed-order sum of a token's rows in the combine scratch (last step of launch_fused_experts), for other expert
+// kernels that leave the same scratch; reads scratch, topk_ids, experts_map, E, T, topk, H, y, y_fp32 of `m`.
+int launch_moe_combine(const MoeParams& m, int wt, cudaStream_t s);
 
 // tcgen05 expert GEMMs (moe_umma.cu): gather of the routed token rows into position order, and one grouped GEMM
 // (mode 1: gate/up + SiLU*up into the [position, I] activation; mode 2: routing-weighted fp32 rows per slot).

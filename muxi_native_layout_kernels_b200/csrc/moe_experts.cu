@@ -525,6 +525,8 @@ int launch_fused_experts(const MoeParams& m0, cudaStream_t s) {
     return launch_combine(m, wt, s);
 }
 
+int launch_moe_combine(const MoeParams& m, int wt, cudaStream_t s) { return launch_combine(m, wt, s); }
+
 // ---------------------------------------------------------------------------------------------------------
 // Expert compute for callers that cannot allocate device memory.
 //
