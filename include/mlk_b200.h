@@ -365,6 +365,33 @@ int mlk_fused_experts_compute_w4(const void* w1, const void* w1_scales, const vo
                                  int experts_map_len, void* workspace, int64_t workspace_bytes, int32_t* status,
                                  mlk_stream_t s);
 
+/* ---- router balance (no counterpart in the reference) ---------------------------------------------------------- */
+
+/* Balance loss of the router, per-expert counts, and the gradient of the loss with respect to the logits:
+ *   p = softmax(logits) (score_fun 0) or sigmoid(logits) / their sum (1), per token;
+ *   c[b,e] = picks topk_ids[t,j] == e by the counted tokens of sequence b, n_b = counted tokens of b;
+ *   loss = coef / sequences * sum_b num_experts / (topK n_b^2) * sum_e c[b,e] sum_{t in b} p[t,e]   (n_b = 0 adds 0);
+ *   counts[e] = sum_b c[b,e].
+ * logits [tokens, num_experts], dtype 0 / 1 / 3 = bf16 / fp16 / fp32, num_experts <= 1024.  topk_ids int32 [tokens, topK], ids
+ * outside [0, num_experts) count nowhere.  token_mask: bytes [tokens], 0 = not counted (NULL = all).  cu_seqlens: int32
+ * [sequences + 1], not decreasing, tokens outside [cu[0], cu[sequences]) belong to no sequence; NULL = one sequence of all
+ * tokens.  Logits of tokens that are not counted are not read and get the gradient 0; a token whose logits are all -inf
+ * has p = 0.  dprob: fp32 [sequences, num_experts], receives d loss / d p (what mlk_router_balance_grad reads).  grad:
+ * NULL, or [tokens, num_experts] in the logits' type, receives d loss / d logits.  Sums in fp32 in a fixed order.
+ * workspace: mlk_router_balance_workspace_bytes(...) bytes on the current device, contents irrelevant. */
+int64_t mlk_router_balance_workspace_bytes(int tokens, int num_experts, int sequences);
+int mlk_router_balance_loss(const void* logits, const int32_t* topk_ids, const void* token_mask, const int32_t* cu_seqlens,
+                            int tokens, int num_experts, int topK, int sequences, int score_fun, float coef, int dtype,
+                            float* loss, int32_t* counts, float* dprob, void* grad, void* workspace,
+                            int64_t workspace_bytes, mlk_stream_t s);
+/* grad = *grad_loss (device scalar, NULL = 1) * d loss / d logits, from the dprob of the call above. */
+int mlk_router_balance_grad(const void* logits, const void* token_mask, const int32_t* cu_seqlens, int tokens, int num_experts,
+                            int sequences, int score_fun, int dtype, const float* dprob, const float* grad_loss, void* grad,
+                            mlk_stream_t s);
+/* counts[e] = number of topk_ids == e among the tokens whose mask byte is not 0 (NULL = all). */
+int mlk_expert_counts(const int32_t* topk_ids, const void* token_mask, int tokens, int topK, int num_experts, int32_t* counts,
+                      mlk_stream_t s);
+
 /* ---- expert-parallel token exchange (no counterpart in the reference, which is single-GPU) ------------------ */
 
 /* out[i,:] = x[idx[i],:] for n_rows rows of `hidden` 16-bit elements (hidden % 8 == 0); an index outside

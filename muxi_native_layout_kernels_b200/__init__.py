@@ -6,8 +6,10 @@ Importing fails if the CUDA library has not been built: there is no fallback pat
 """
 from .ext import *  # noqa: F401,F403
 from .ext import __all__ as _ext_all
+from .balance import *  # noqa: F401,F403
+from .balance import __all__ as _balance_all
 from .w4 import *  # noqa: F401,F403
 from .w4 import __all__ as _w4_all
-from . import ext, muxi_moe_planC, parallel, utils, w4  # noqa: F401
+from . import balance, ext, muxi_moe_planC, parallel, utils, w4  # noqa: F401
 
-__all__ = list(_ext_all) + list(_w4_all) + ["w4"] + ["ext", "muxi_moe_planC", "parallel", "utils"]
+__all__ = list(_ext_all) + list(_w4_all) + list(_balance_all) + ["balance", "w4"] + ["ext", "muxi_moe_planC", "parallel", "utils"]

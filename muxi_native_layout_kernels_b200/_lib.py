@@ -71,6 +71,11 @@ PROTOTYPES = {
     "mlk_fused_experts_compute_w4": (c_int, [c_vp, c_vp, c_vp, c_int, c_vp, c_vp, c_vp, c_int, c_vp, c_int, c_int, c_int,
                                              c_int, c_int, c_vp, c_vp, c_vp, c_int, c_int, c_vp, c_int, c_vp, c_i64, c_vp,
                                              c_vp]),
+    "mlk_router_balance_workspace_bytes": (c_i64, [c_int, c_int, c_int]),
+    "mlk_router_balance_loss": (c_int, [c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int, c_f32, c_int, c_vp, c_vp,
+                                        c_vp, c_vp, c_vp, c_i64, c_vp]),
+    "mlk_router_balance_grad": (c_int, [c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_vp]),
+    "mlk_expert_counts": (c_int, [c_vp, c_vp, c_int, c_int, c_int, c_vp, c_vp]),
     "mlk_ep_reduce_flag_bytes": (c_i64, []),
     "mlk_ep_reduce_recv_bytes": (c_i64, [c_int, c_i64, c_int]),
     "mlk_ep_reduce_shares": (c_int, [c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_i64, c_int, c_int, c_vp, c_vp]),

@@ -38,6 +38,7 @@ SOURCES = [
     "moe_decode.cu",
     "ep_reduce.cu",
     "moe_exchange.cu",
+    "moe_balance.cu",
     "w4_pack.cu",
     "w4_dense.cu",
     "w4_mma.cu",

@@ -7,6 +7,7 @@
 
 #include "dense.cuh"
 #include "moe.cuh"
+#include "moe_balance.cuh"
 #include "selector.h"
 #include "status.h"
 #include "w4.cuh"
@@ -566,6 +567,40 @@ int mlk_fused_experts_compute_w4(const void* w1, const void* w1_scales, const vo
     p.experts_map = experts_map; p.experts_map_len = experts_map_len;
     p.workspace = workspace; p.workspace_bytes = workspace_bytes; p.status = status;
     return guarded([&] { return launch_w4_experts(p, (cudaStream_t)s); });
+}
+
+// ---- router balance --------------------------------------------------------------------------------------------
+
+int64_t mlk_router_balance_workspace_bytes(int tokens, int num_experts, int sequences) {
+    return balance_workspace_bytes(tokens, num_experts, sequences);
+}
+
+int mlk_router_balance_loss(const void* logits, const int32_t* topk_ids, const void* token_mask, const int32_t* cu_seqlens,
+                            int tokens, int num_experts, int topK, int sequences, int score_fun, float coef, int dtype,
+                            float* loss, int32_t* counts, float* dprob, void* grad, void* workspace,
+                            int64_t workspace_bytes, mlk_stream_t s) {
+    BalanceParams b{logits, topk_ids, reinterpret_cast<const uint8_t*>(token_mask), cu_seqlens, tokens, num_experts, topK,
+                    sequences, score_fun, dtype, coef, loss, counts, dprob, nullptr, grad};
+    return guarded([&] {
+        if (int st = launch_balance_loss(b, workspace, workspace_bytes, (cudaStream_t)s)) return st;
+        return grad ? launch_balance_grad(b, (cudaStream_t)s) : (int)kOk;
+    });
+}
+
+int mlk_router_balance_grad(const void* logits, const void* token_mask, const int32_t* cu_seqlens, int tokens, int num_experts,
+                            int sequences, int score_fun, int dtype, const float* dprob, const float* grad_loss, void* grad,
+                            mlk_stream_t s) {
+    BalanceParams b{logits, nullptr, reinterpret_cast<const uint8_t*>(token_mask), cu_seqlens, tokens, num_experts, 1,
+                    sequences, score_fun, dtype, 0.f, nullptr, nullptr, const_cast<float*>(dprob), grad_loss, grad};
+    return guarded([&] { return launch_balance_grad(b, (cudaStream_t)s); });
+}
+
+int mlk_expert_counts(const int32_t* topk_ids, const void* token_mask, int tokens, int topK, int num_experts, int32_t* counts,
+                      mlk_stream_t s) {
+    return guarded([&] {
+        return launch_expert_counts(topk_ids, reinterpret_cast<const uint8_t*>(token_mask), tokens, topK, num_experts, counts,
+                                    (cudaStream_t)s);
+    });
 }
 
 }  // extern "C"

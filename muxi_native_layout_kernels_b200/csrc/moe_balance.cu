@@ -1,0 +1,504 @@
+// Balance loss of a mixture layer's router, per-expert counts, and the gradient with respect to the router logits.
+//
+//   p[t, e]  = softmax(l_t)_e, or sigmoid(l_te) / sum_f sigmoid(l_tf)
+//   c[b, e]  = picks of expert e by the counted tokens of sequence b (ids[t, j] == e),   n_b = counted tokens of b
+//   loss     = coef / B * sum_b E / (topk n_b^2) * sum_e c[b, e] * sum_{t in b} p[t, e]      (n_b = 0 adds nothing)
+//   u[b, e]  = coef E c[b, e] / (B topk n_b^2)                                               = d loss / d p[t, e]
+//   d loss / d l_te = p_te (u_be - sum_f p_tf u_bf)           (times 1 - sigmoid(l_te) for the sigmoid scores)
+//
+// The counts are known only when every token has been seen, so the logits are read twice: three kernels,
+//   partial   blocks over runs of R tokens; a run crosses sequence borders freely, each (run i, sequence b) that meet
+//             leaves one record (sums of p in fp32, counts, tokens) at index i + b, which is unique because both only
+//             grow along the tokens: no buffer has to be cleared and no float is added by an atomic
+//   finish    one cluster of eight CTAs, a slice of the experts each: records -> counts, u, loss, in a fixed order
+//   grad      the runs again: p recomputed, u in, gradient out
+// What bounds it: at large T the logits (two reads, one write); below some thousand tokens the three launches.
+// A row's 16-byte loads are spread over as few lanes as cover it (8 experts in bf16: one lane per token), so that a warp
+// holds up to 32 tokens and the reductions over experts take log2(lanes per row) shuffles.
+#include <algorithm>
+#include <cmath>
+
+#include "common.cuh"
+#include "moe_balance.cuh"
+#include "status.h"
+
+namespace mlk {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kFinishThreads = 512;
+constexpr int kFinishCtas = 8;
+constexpr int kF32 = 3;          // dtype code of fp32 logits in this file
+
+struct Params {
+    const void* logits;
+    const int32_t* ids;          // [T, topk]
+    const uint8_t* mask;         // [T] or null
+    const int32_t* cu;           // [B + 1] or null (one sequence, all tokens)
+    int T, E, topk, B, score_fun;
+    int R;                       // tokens per run
+    int lpr;                     // lanes per row
+    float coef;
+    float* P;                    // records
+    int32_t* C;
+    int32_t* N;
+    float* u;                    // [B, E]
+    float* loss;
+    int32_t* counts;             // [E]
+    const float* grad_loss;      // scalar or null = 1
+    void* grad;                  // [T, E]
+};
+
+__device__ __forceinline__ int seq_start(const Params& p, int b) {
+    return p.cu == nullptr ? (b == 0 ? 0 : p.T) : min(max(p.cu[b], 0), p.T);
+}
+
+// first sequence that ends behind token t (B: none)
+__device__ int seq_of(const Params& p, int t) {
+    if (p.cu == nullptr) return 0;
+    int lo = 0, hi = p.B;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (seq_start(p, mid + 1) > t) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
+
+template <int T>
+struct Elem;
+template <> struct Elem<kBF16> { using type = uint16_t; };
+template <> struct Elem<kFP16> { using type = uint16_t; };
+template <> struct Elem<kF32> { using type = float; };
+
+template <int DT>
+__device__ __forceinline__ float as_float(typename Elem<DT>::type v) {
+    if constexpr (DT == kF32) return v;
+    else if constexpr (DT == kBF16) return __uint_as_float((uint32_t)v << 16);
+    else return __half2float(__ushort_as_half(v));
+}
+template <int DT>
+__device__ __forceinline__ typename Elem<DT>::type from_float(float v) {
+    if constexpr (DT == kF32) return v;
+    else if constexpr (DT == kBF16) return __bfloat16_as_ushort(__float2bfloat16_rn(v));
+    else return __half_as_ushort(__float2half_rn(v));
+}
+
+__device__ __forceinline__ float group_sum(float v, int lpr) {
+    for (int o = lpr >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    return v;
+}
+__device__ __forceinline__ float group_max(float v, int lpr) {
+    for (int o = lpr >> 1; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+    return v;
+}
+
+// Column of value i of a lane: J vectors of V neighbouring experts, lpr * V apart.
+template <int V>
+__device__ __forceinline__ int column(int i, int sub, int lpr) { return (i / V) * (lpr * V) + sub * V + i % V; }
+
+template <int DT, int V, int J>
+__device__ __forceinline__ void load_row(const Params& p, long long row, int sub, bool live, float (&x)[V * J]) {
+    using E = typename Elem<DT>::type;
+    const E* base = reinterpret_cast<const E*>(p.logits) + row * p.E;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        const int c = j * (p.lpr * V) + sub * V;
+        E v[V];
+        if (live && c < p.E) {                  // V divides E: a vector is in or out as a whole
+            if constexpr (V * sizeof(E) == 16) *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(base + c);
+            else if constexpr (V * sizeof(E) == 8) *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(base + c);
+            else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[i] = base[c + i];
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) x[j * V + i] = as_float<DT>(v[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) x[j * V + i] = -INFINITY;     // exp and sigmoid give 0
+        }
+    }
+}
+
+// Scores of a row in place; `one_minus`: 1 - sigmoid for the gradient (sigmoid scores).  A row whose logits are all -inf
+// has no distribution: its scores are 0.
+template <int N, bool GRAD>
+__device__ __forceinline__ void scores(const Params& p, float (&x)[N], float (&one_minus)[GRAD ? N : 1]) {
+    float s = 0.f;
+    if (p.score_fun == 0) {
+        float m = x[0];
+#pragma unroll
+        for (int i = 1; i < N; ++i) m = fmaxf(m, x[i]);
+        m = group_max(m, p.lpr);
+        if (m == -INFINITY) m = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) s += x[i] = expf(x[i] - m);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            // both forms from exp(-|x|), which cannot overflow
+            const float e = expf(-fabsf(x[i])), d = 1.f / (1.f + e);
+            const float pos = d, neg = e * d;
+            if constexpr (GRAD) one_minus[i] = x[i] >= 0.f ? neg : pos;
+            s += x[i] = x[i] != x[i] ? x[i] : (x[i] >= 0.f ? pos : neg);
+        }
+    }
+    s = group_sum(s, p.lpr);
+    const float inv = s == 0.f ? 0.f : 1.f / s;
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] *= inv;
+}
+
+template <int DT, int V, int J>
+__global__ void __launch_bounds__(kThreads) balance_partial_kernel(const Params p) {
+    constexpr int N = V * J;
+    extern __shared__ __align__(16) uint8_t smem[];
+    float* const sP = reinterpret_cast<float*>(smem);                       // [warps][E]
+    int32_t* const sC = reinterpret_cast<int32_t*>(sP + (kThreads / 32) * p.E);
+    __shared__ int sN[kThreads / 32];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, sub = lane & (p.lpr - 1);
+    const int rows_per_warp = 32 / p.lpr, group = lane / p.lpr;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int begin = blockIdx.x * p.R, end = min(begin + p.R, p.T);
+    for (int b = seq_of(p, begin); b < p.B; ++b) {
+        const int s0 = seq_start(p, b), s1 = seq_start(p, b + 1);
+        if (s0 >= end) break;
+        const int a = max(s0, begin), z = min(s1, end);
+        if (a >= z) continue;                                               // an empty sequence has no record
+        for (int e = tid; e < p.E; e += kThreads) sC[e] = 0;
+        __syncthreads();
+        float acc[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] = 0.f;
+        int n = 0;
+        for (int r0 = a + warp * rows_per_warp; r0 < z; r0 += (kThreads / 32) * rows_per_warp) {
+            const int row = r0 + group;
+            const bool live = row < z && (p.mask == nullptr || p.mask[row] != 0);
+            float x[N], unused[1];
+            load_row<DT, V, J>(p, row, sub, live, x);
+            if (live) {
+                for (int j = sub; j < p.topk; j += p.lpr) {
+                    const int e = p.ids[(long long)row * p.topk + j];
+                    if (e >= 0 && e < p.E) atomicAdd(&sC[e], 1);
+                }
+                n += sub == 0;
+            }
+            scores<N, false>(p, x, unused);
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[i] += x[i];
+        }
+        // the warp's rows, then the warps, in a fixed order
+        for (int o = 16; o >= p.lpr; o >>= 1)
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[i] += __shfl_xor_sync(0xFFFFFFFFu, acc[i], o);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xFFFFFFFFu, n, o);
+        if (group == 0)
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int c = column<V>(i, sub, p.lpr);
+                if (c < p.E) sP[warp * p.E + c] = acc[i];
+            }
+        if (lane == 0) sN[warp] = n;
+        __syncthreads();
+        const long long rec = (long long)blockIdx.x + b;
+        for (int e = tid; e < p.E; e += kThreads) {
+            float v = sP[e];
+#pragma unroll
+            for (int w = 1; w < kThreads / 32; ++w) v += sP[w * p.E + e];
+            p.P[rec * p.E + e] = v;
+            p.C[rec * p.E + e] = sC[e];
+        }
+        if (tid == 0) {
+            int v = 0;
+            for (int w = 0; w < kThreads / 32; ++w) v += sN[w];
+            p.N[rec] = v;
+        }
+        __syncthreads();
+    }
+}
+
+// One cluster: CTA r owns the experts [r * cw, (r + 1) * cw).  A thread is (expert column, part): `parts` of them share
+// the records of the sequences of a round, `per` threads to a sequence.
+__global__ void __cluster_dims__(kFinishCtas, 1, 1) __launch_bounds__(kFinishThreads) balance_finish_kernel(const Params p, int cw) {
+    __shared__ float sP[kFinishThreads];
+    __shared__ int sC[kFinishThreads], sN[kFinishThreads];
+    __shared__ float sL[kFinishThreads];
+    __shared__ float total;
+    const int tid = threadIdx.x, r = blockIdx.x;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int col = tid % cw, part = tid / cw, parts = kFinishThreads / cw;
+    const int e = r * cw + col;
+    const bool mine = part < parts && e < p.E;
+    const int per = max(1, parts / p.B), round = parts / per;       // threads of a column per sequence, sequences per round
+    const int sub = part % per, which = part / per;
+    float loss = 0.f;
+    int count = 0;
+    for (int b0 = 0; b0 < p.B; b0 += round) {
+        const int b = b0 + which;
+        float P = 0.f;
+        int C = 0, n = 0;
+        if (mine && which < round && b < p.B) {
+            const int s0 = seq_start(p, b), s1 = seq_start(p, b + 1);
+            if (s0 < s1) {
+                const int i1 = (s1 - 1) / p.R;
+#pragma unroll 4
+                for (int i = s0 / p.R + sub; i <= i1; i += per) {
+                    const long long rec = (long long)i + b;
+                    P += p.P[rec * p.E + e];
+                    C += p.C[rec * p.E + e];
+                    n += p.N[rec];
+                }
+            }
+        }
+        if (per > 1) {
+            sP[tid] = P; sC[tid] = C; sN[tid] = n;
+            __syncthreads();
+            if (mine && which < round && b < p.B && sub == 0)
+                for (int k = 1; k < per; ++k) {
+                    P += sP[tid + k * cw];
+                    C += sC[tid + k * cw];
+                    n += sN[tid + k * cw];
+                }
+            __syncthreads();
+        }
+        if (mine && which < round && b < p.B && sub == 0) {
+            // n_b * n_b in fp32: 24 bits are enough for a scale factor
+            const float u = n > 0 ? p.coef * (float)p.E * (float)C / ((float)p.B * (float)p.topk * (float)n * (float)n) : 0.f;
+            p.u[(long long)b * p.E + e] = u;
+            loss += u * P;
+            count += C;
+        }
+    }
+    sL[tid] = loss;
+    sC[tid] = count;
+    __syncthreads();
+    if (tid < cw && e < p.E) {
+        int c = 0;
+        for (int k = 0; k < parts; ++k) c += sC[tid + k * cw];
+        p.counts[e] = c;
+    }
+    for (int o = kFinishThreads / 2; o > 0; o >>= 1) {
+        if (tid < o) sL[tid] += sL[tid + o];
+        __syncthreads();
+    }
+    if (tid == 0) total = sL[0];
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (r == 0 && tid == 0) {
+        float v = 0.f;
+        for (int q = 0; q < kFinishCtas; ++q) {
+            uint32_t at;
+            float x;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(&total)), "r"(q));
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(at) : "memory");
+            v += x;
+        }
+        p.loss[0] = v;
+    }
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <int DT, int V, int J>
+__global__ void __launch_bounds__(kThreads) balance_grad_kernel(const Params p) {
+    constexpr int N = V * J;
+    using E = typename Elem<DT>::type;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, sub = lane & (p.lpr - 1);
+    const int rows_per_warp = 32 / p.lpr, group = lane / p.lpr;
+    pdl_wait();
+    pdl_launch_dependents();
+    const float g = p.grad_loss ? *p.grad_loss : 1.f;
+    for (long long r0 = ((long long)blockIdx.x * (kThreads / 32) + warp) * rows_per_warp; r0 < p.T;
+         r0 += (long long)gridDim.x * (kThreads / 32) * rows_per_warp) {
+        const int row = (int)r0 + group;
+        bool live = row < p.T && (p.mask == nullptr || p.mask[row] != 0);
+        int b = 0;
+        if (live && p.cu != nullptr) {
+            b = seq_of(p, row);
+            live = b < p.B && seq_start(p, b) <= row;
+        }
+        float x[N], one_minus[N];
+        load_row<DT, V, J>(p, row, sub, live, x);
+        scores<N, true>(p, x, one_minus);
+        const float* const ub = p.u + (long long)b * p.E;
+        float u[N], dot = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int c = column<V>(i, sub, p.lpr);
+            u[i] = live && c < p.E ? ub[c] : 0.f;
+            dot += x[i] * u[i];
+        }
+        dot = group_sum(dot, p.lpr);
+        if (row < p.T) {
+            E* const out = reinterpret_cast<E*>(p.grad) + (long long)row * p.E;
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const int c = j * (p.lpr * V) + sub * V;
+                if (c >= p.E) continue;
+                E v[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    float d = live ? g * (x[j * V + i] * (u[j * V + i] - dot)) : 0.f;
+                    if (p.score_fun == 1 && live) d *= one_minus[j * V + i];
+                    v[i] = from_float<DT>(d);
+                }
+                if constexpr (V * sizeof(E) == 16) *reinterpret_cast<uint4*>(out + c) = *reinterpret_cast<uint4*>(v);
+                else if constexpr (V * sizeof(E) == 8) *reinterpret_cast<uint2*>(out + c) = *reinterpret_cast<uint2*>(v);
+                else {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) out[c + i] = v[i];
+                }
+            }
+        }
+    }
+}
+
+// Counts alone: one counter block per CTA in shared memory, integer atomics into the cleared result.
+__global__ void __launch_bounds__(kThreads) expert_counts_kernel(const int32_t* __restrict__ ids, const uint8_t* __restrict__ mask,
+                                                                long long n, int topk, int E, int32_t* __restrict__ counts) {
+    extern __shared__ int32_t c[];
+    for (int e = threadIdx.x; e < E; e += kThreads) c[e] = 0;
+    pdl_wait();
+    pdl_launch_dependents();
+    __syncthreads();
+    for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < n; i += (long long)gridDim.x * kThreads) {
+        const int e = ids[i];
+        if (e >= 0 && e < E && (mask == nullptr || mask[i / topk] != 0)) atomicAdd(&c[e], 1);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < E; e += kThreads)
+        if (c[e] != 0) atomicAdd(&counts[e], c[e]);
+}
+
+struct Plan {
+    int v, j, lpr, runs, R;
+};
+
+Plan plan(int T, int E, int elem, bool aligned) {
+    Plan q{};
+    q.v = elem == 2 && E % 8 == 0 ? 8 : (E % 4 == 0 ? 4 : 1);
+    if (!aligned) q.v = 1;
+    const int vectors = (E + q.v - 1) / q.v;
+    q.lpr = 1;
+    while (q.lpr < 32 && q.lpr < vectors) q.lpr *= 2;
+    q.j = (vectors + q.lpr - 1) / q.lpr;
+    // two runs per SM, at least one pass of a block's warps each
+    const int rows = (kThreads / 32) * (32 / q.lpr);
+    const int want = 2 * sm_count();
+    q.R = std::max(rows, ((T + want - 1) / want + rows - 1) / rows * rows);
+    q.runs = (T + q.R - 1) / q.R;
+    return q;
+}
+
+using Kern = void (*)(Params);
+template <int DT, bool GRAD, int V, int J>
+constexpr Kern kernel() {
+    if constexpr (GRAD) return balance_grad_kernel<DT, V, J>;
+    else return balance_partial_kernel<DT, V, J>;
+}
+template <int DT, bool GRAD>
+Kern pick(int v, int j) {
+    if (DT != kF32 && v == 8) return j == 1 ? kernel<DT, GRAD, DT == kF32 ? 4 : 8, 1>() : kernel<DT, GRAD, DT == kF32 ? 4 : 8, 4>();
+    if (v == 4) return j == 1 ? kernel<DT, GRAD, 4, 1>() : (j == 2 ? kernel<DT, GRAD, 4, 2>() : kernel<DT, GRAD, 4, 8>());
+    return j <= 2 ? kernel<DT, GRAD, 1, 2>() : kernel<DT, GRAD, 1, 32>();
+}
+template <bool GRAD>
+Kern pick(int dt, int v, int j) {
+    return dt == kF32 ? pick<kF32, GRAD>(v, j) : (dt == kFP16 ? pick<kFP16, GRAD>(v, j) : pick<kBF16, GRAD>(v, j));
+}
+
+template <class K, class... A>
+int launch(const char* what, K kern, int grid, int threads, size_t smem, cudaStream_t s, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    cfg.attrs = attr;
+    cfg.numAttrs = launch_attrs(attr, 1);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+    if (e != cudaSuccess) return fail(kCudaError, "%s launch: %s", what, cudaGetErrorString(e));
+    return kOk;
+}
+
+int check(const BalanceParams& b, const char* who) {
+    if (b.T < 0 || b.B < 1 || b.topk < 1) return fail(kInvalidArg, "%s: bad sizes", who);
+    if (b.E < 1 || b.E > kBalanceMaxExperts) return fail(kUnsupported, "%s: 1 <= experts <= %d (got %d)", who, kBalanceMaxExperts, b.E);
+    if (b.dtype < 0 || b.dtype > 3 || b.dtype == kE4M3) return fail(kInvalidArg, "%s: logits must be bf16, fp16 or fp32", who);
+    if (b.score_fun != 0 && b.score_fun != 1) return fail(kInvalidArg, "%s: score_fun must be 0 (softmax) or 1 (sigmoid)", who);
+    if (b.B > 1 && !b.cu_seqlens) return fail(kInvalidArg, "%s: more than one sequence needs cu_seqlens", who);
+    if (b.T > 0 && !b.logits) return fail(kInvalidArg, "%s: null pointer", who);
+    if ((long long)b.B + b.T > 0x3FFFFFFF) return fail(kUnsupported, "%s: too many tokens or sequences", who);
+    return kOk;
+}
+
+Params params(const BalanceParams& b, const Plan& q) {
+    Params p{};
+    p.logits = b.logits; p.ids = b.ids; p.mask = b.mask; p.cu = b.cu_seqlens;
+    p.T = b.T; p.E = b.E; p.topk = b.topk; p.B = b.B; p.score_fun = b.score_fun; p.coef = b.coef;
+    p.R = q.R; p.lpr = q.lpr;
+    p.u = b.u; p.loss = b.loss; p.counts = b.counts; p.grad_loss = b.grad_loss; p.grad = b.grad;
+    return p;
+}
+
+Plan plan_of(const BalanceParams& b) {
+    const bool aligned = (((uintptr_t)b.logits | (uintptr_t)b.grad) & 15) == 0;
+    return plan(b.T, b.E, b.dtype == kF32 ? 4 : 2, aligned);
+}
+
+}  // namespace
+
+long long balance_workspace_bytes(int T, int E, int B) {
+    if (T < 0 || E < 1 || B < 1) return 0;
+    // the most runs any plan makes: 2 per SM, and never more than tokens
+    const long long records = (long long)std::min(T, 2 * sm_count() + 1) + B;
+    return (records * E * 2 + records) * 4;
+}
+
+int launch_balance_loss(const BalanceParams& b, void* workspace, long long workspace_bytes, cudaStream_t s) {
+    if (int st = check(b, "router_balance_loss")) return st;
+    if (!b.loss || !b.counts || !b.u || (b.T > 0 && (!b.ids || !workspace))) return fail(kInvalidArg, "router_balance_loss: null pointer");
+    const Plan q = plan_of(b);
+    Params p = params(b, q);
+    const long long records = (long long)q.runs + b.B;
+    if (b.T > 0 && workspace_bytes < (records * b.E * 2 + records) * 4)
+        return fail(kInvalidArg, "router_balance_loss: workspace holds %lld bytes, needs %lld", workspace_bytes, (records * b.E * 2 + records) * 4);
+    p.P = reinterpret_cast<float*>(workspace);
+    p.C = reinterpret_cast<int32_t*>(p.P + records * b.E);
+    p.N = p.C + records * b.E;
+    if (b.T > 0) {
+        const size_t smem = (size_t)(kThreads / 32 + 1) * b.E * 4;
+        if (int st = launch("router_balance_loss", pick<false>(b.dtype, q.v, q.j), q.runs, kThreads, smem, s, p)) return st;
+    }
+    return launch("router_balance_loss (finish)", balance_finish_kernel, kFinishCtas, kFinishThreads, 0, s, p,
+                  (b.E + kFinishCtas - 1) / kFinishCtas);
+}
+
+int launch_balance_grad(const BalanceParams& b, cudaStream_t s) {
+    if (int st = check(b, "router_balance_grad")) return st;
+    if (b.T == 0) return kOk;
+    if (!b.u || !b.grad) return fail(kInvalidArg, "router_balance_grad: null pointer");
+    const Plan q = plan_of(b);
+    const int rows = (kThreads / 32) * (32 / q.lpr);
+    const int grid = std::min((b.T + rows - 1) / rows, 8 * sm_count());
+    return launch("router_balance_grad", pick<true>(b.dtype, q.v, q.j), grid, kThreads, 0, s, params(b, q));
+}
+
+int launch_expert_counts(const int32_t* ids, const uint8_t* mask, int T, int topk, int E, int32_t* counts, cudaStream_t s) {
+    if (T < 0 || topk < 1) return fail(kInvalidArg, "expert_counts: bad sizes");
+    if (E < 1 || E > kBalanceMaxExperts) return fail(kUnsupported, "expert_counts: 1 <= experts <= %d (got %d)", kBalanceMaxExperts, E);
+    if (!counts || (T > 0 && !ids)) return fail(kInvalidArg, "expert_counts: null pointer");
+    cudaError_t e = cudaMemsetAsync(counts, 0, (size_t)E * 4, s);
+    if (e != cudaSuccess) return fail(kCudaError, "expert_counts: %s", cudaGetErrorString(e));
+    if (T == 0) return kOk;
+    const long long n = (long long)T * topk;
+    const int grid = (int)std::min<long long>((n + 4 * kThreads - 1) / (4 * kThreads), 2LL * sm_count());
+    return launch("expert_counts", expert_counts_kernel, grid, kThreads, (size_t)E * 4, s, ids, mask, n, topk, E, counts);
+}
+
+}  // namespace mlk
