@@ -14,10 +14,9 @@ int launch_w4_dense(const W4DenseParams& p, cudaStream_t s) {
     if (p.k % p.w.group != 0) return fail(kInvalidArg, "gemm_layoutA_w4: k = %d is not whole groups of %d", p.k, p.w.group);
     if (p.dtype != kBF16 && p.dtype != kFP16) return fail(kInvalidArg, "gemm_layoutA_w4: activations must be bf16 or fp16");
     if (!p.w.q || !p.w.s || (p.n > 0 && (!p.X || !p.C))) return fail(kInvalidArg, "gemm_layoutA_w4: null pointer");
-    if (((uintptr_t)p.w.q | (uintptr_t)p.X | (uintptr_t)p.C) & 15)
-        return fail(kInvalidArg, "gemm_layoutA_w4: A, B and C must be 16-byte aligned");
-    if (((uintptr_t)p.w.s & 3) || ((uintptr_t)p.w.z & 1) || ((uintptr_t)p.bias & 1))
-        return fail(kInvalidArg, "gemm_layoutA_w4: scales, zeros or bias are not aligned");
+    if (((uintptr_t)p.w.q | (uintptr_t)p.w.s | (uintptr_t)p.w.z | (uintptr_t)p.X | (uintptr_t)p.C) & 15)
+        return fail(kInvalidArg, "gemm_layoutA_w4: A, scales, zeros, B and C must be 16-byte aligned");
+    if ((uintptr_t)p.bias & 1) return fail(kInvalidArg, "gemm_layoutA_w4: bias is not aligned");
     if (p.n == 0) return kOk;
 
     W4KernelParams g{};
@@ -26,15 +25,11 @@ int launch_w4_dense(const W4DenseParams& p, cudaStream_t s) {
     g.out_tiles = g.mat_tiles = p.m / 16;
     g.k = p.k;
     const int nt = p.n <= 8 ? 1 : 2, block = 8 * nt;
-    const int sk = w4_mma_split((long long)g.out_tiles / 2 * ((p.n + block - 1) / block), p.k / 64);
-    // a launch holds at most 65535 token blocks
-    for (long long n0 = 0; n0 < p.n; n0 += 65535LL * block) {
-        g.X = reinterpret_cast<const uint8_t*>(p.X) + n0 * p.k * 2;
-        g.C = reinterpret_cast<uint8_t*>(p.C) + n0 * p.m * 2;
-        g.n = (int)std::min<long long>(p.n - n0, 65535LL * block);
-        if (int st = launch_w4_mma(0, p.dtype, g, p.w, (g.n + block - 1) / block, nt, sk, s)) return st;
-    }
-    return kOk;
+    g.X = p.X;
+    g.C = p.C;
+    g.n = p.n;
+    const int items = (p.n + block - 1) / block;
+    return launch_w4_mma(0, p.dtype, g, p.w, items, items, nt, s);
 }
 
 }  // namespace mlk

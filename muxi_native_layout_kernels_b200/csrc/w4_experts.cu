@@ -5,6 +5,7 @@
 // slot order with one rounding.  The activation between the two products is rounded to the 16-bit activation type, as in
 // the 16-bit and e4m3 expert kernels.
 #include <algorithm>
+#include <cmath>
 
 #include "moe.cuh"
 #include "w4_kernels.cuh"
@@ -43,8 +44,8 @@ int check_weights(const W4Weights& w, long long k, const char* name) {
     if (w.group != 32 && w.group != 64 && w.group != 128)
         return fail(kInvalidArg, "fused_experts_compute_w4: %s: groups of 32, 64 or 128 (got %d)", name, w.group);
     if (k % w.group != 0) return fail(kInvalidArg, "fused_experts_compute_w4: %s: k = %lld is not whole groups of %d", name, k, w.group);
-    if (((uintptr_t)w.q & 15) || ((uintptr_t)w.s & 3) || ((uintptr_t)w.z & 1))
-        return fail(kInvalidArg, "fused_experts_compute_w4: %s is not aligned", name);
+    if (((uintptr_t)w.q | (uintptr_t)w.s | (uintptr_t)w.z) & 15)
+        return fail(kInvalidArg, "fused_experts_compute_w4: %s, its scales and zeros must be 16-byte aligned", name);
     return kOk;
 }
 
@@ -80,6 +81,8 @@ int launch_w4_experts(const W4ExpertsParams& p, cudaStream_t s) {
 
     const int nt = slots <= 4LL * p.E ? 1 : 2, block = 8 * nt;
     const int items = (int)max_items(slots, p.E, block);
+    // experts that get a slot when all are as likely, and the further items of full ones: what the grid is planned for
+    const int likely = std::min(items, std::max(1, (int)(p.E * (1.0 - std::exp(-(double)slots / p.E)) + (double)slots / block * 0.5)));
     if (int st = launch_moe_align(p.T, p.E, p.topk, 1, p.topk_ids, sorted, reinterpret_cast<int32_t*>(ws + l.cumsum),
                                   reinterpret_cast<int32_t*>(ws + l.nblocks), reinterpret_cast<int32_t*>(ws + l.block_expert),
                                   p.experts_map, p.experts_map_len, s, worklist, block))
@@ -95,12 +98,12 @@ int launch_w4_experts(const W4ExpertsParams& p, cudaStream_t s) {
     g.k = p.H;
     g.out_tiles = p.I / 16;
     g.mat_tiles = 2 * p.I / 16;
-    if (int st = launch_w4_mma(1, p.dtype, g, p.w1, items, nt, w4_mma_split((long long)g.out_tiles * items, p.H / 64), s)) return st;
+    if (int st = launch_w4_mma(1, p.dtype, g, p.w1, items, likely, nt, s)) return st;
     g.X = act;
     g.C = scratch;
     g.k = p.I;
     g.out_tiles = g.mat_tiles = p.H / 16;
-    if (int st = launch_w4_mma(2, p.dtype, g, p.w2, items, nt, w4_mma_split((long long)g.out_tiles / 2 * items, p.I / 64), s)) return st;
+    if (int st = launch_w4_mma(2, p.dtype, g, p.w2, items, likely, nt, s)) return st;
 
     MoeParams m{};
     m.scratch = scratch; m.topk_ids = p.topk_ids; m.experts_map = p.experts_map; m.experts_map_len = p.experts_map_len;

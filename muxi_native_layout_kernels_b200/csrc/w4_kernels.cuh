@@ -15,7 +15,9 @@ struct W4KernelParams {
     float alpha;
     int out_tiles;              // 16-row tiles of the output (MODE 1: of the gate half)
     int mat_tiles;              // 16-row tiles of one expert's matrix
-    int n, k, kc, groups, group_shift;
+    int n, k, kc, groups;
+    int row_warps;              // warps of a CTA side by side in the rows; the others split k
+    int seg_units;              // units of 128 k of one staging of activations and scales
     // experts
     const int4* worklist;       // [0] = {items,..}; then {expert, first position, slots, first compact position}
     const int32_t* sorted;      // slot id of every position
@@ -29,7 +31,8 @@ __device__ __forceinline__ void store16(void* base, size_t i, float v) {
     else reinterpret_cast<__nv_bfloat16*>(base)[i] = __float2bfloat16_rn(v);
 }
 
-int launch_w4_mma(int mode, int wt, W4KernelParams p, const W4Weights& w, int token_blocks, int nt, int sk, cudaStream_t s);
-int w4_mma_split(long long row_ctas, int kc);
+// items: work items (exact for the dense products, an upper bound for the experts, whose number the device knows);
+// likely_items: what the grid is sized for.
+int launch_w4_mma(int mode, int wt, W4KernelParams p, const W4Weights& w, int items, int likely_items, int nt, cudaStream_t s);
 
 }  // namespace mlk

@@ -9,12 +9,20 @@
 // traffic): 16.8 T weights/s with one column tile of 8 tokens, 11 T with two; HBM delivers 13 T.  More than 16 tokens go
 // to the tcgen05 kernel.
 //
-// A warp owns R tiles of 16 rows and every W-th block of 64 k; the activation fragment of a block (column operand, one
-// 8-byte load per step and 8 tokens) serves all R tiles.  Weights travel through a private ring of each warp in shared
-// memory filled by 16-byte cp.async: a lane copies exactly the bytes that it will read itself, so the ring needs no
-// barrier, costs no registers and keeps 2 to 4 KB per warp in flight.  The warps' partial sums meet in shared memory, the
-// k parts of a cluster in distributed shared memory, both in a fixed order: results do not depend on timing.
+// A warp owns RT tiles of 16 rows and every WK-th unit of 128 k; WR x WK = 8 warps share the rows and the k range of a CTA.
+// The CTA's activations and scales are staged in shared memory once, so that a unit costs one 8-byte shared load per step
+// and 8 tokens for the column operand of all RT tiles.  Weights travel through a private ring of each warp filled by
+// 16-byte cp.async: a lane copies exactly the bytes that it will read itself, so the ring needs no barrier and costs no
+// registers.  The warps' partial sums meet in shared memory, the k parts of a cluster in distributed shared memory, both
+// in a fixed order: results do not depend on timing.
+// Measured and not used: activations and scales fetched by each warp from global memory (21 instead of 14 instructions per
+// word; 28672 x 8192 at 8 tokens 37 instead of 31 us); a persistent grid with an equal run of tiles per SM (31 us there, but
+// 80 instead of 64 us for 33 tokens on 128 small experts); activations kept in registers with the rows streaming past
+// (33 and 85 us: every few tiles all warps have to meet).
 #include <algorithm>
+#include <array>
+#include <cmath>
+#include <map>
 
 #include "umma_common.cuh"
 #include "w4.cuh"
@@ -24,12 +32,21 @@ namespace mlk {
 
 namespace {
 
-constexpr int kWarps = 8;
 constexpr int kTokStride = 20;   // floats between two tokens' 16 rows in the reduction buffer: conflict-free fragments
 
-__device__ __forceinline__ uint2 ld_x(const uint8_t* p) {
+__device__ __forceinline__ uint2 lds8(uint32_t addr) {
     uint2 v;
-    asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ uint32_t lds4(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ uint32_t lds2(uint32_t addr) {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
     return v;
 }
 
@@ -37,28 +54,37 @@ __device__ __forceinline__ void cp_async16_hint(uint32_t dst, const void* src, u
     asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(pol) : "memory");
 }
 
-// first step of a group: the accumulator starts at zero
+// first step of a group: D = A * B
 template <int WT>
 __device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint2 b) {
-    d[0] = d[1] = d[2] = d[3] = 0.f;
-    mma16816<WT>(d, a[0], a[1], a[2], a[3], b.x, b.y);
+    if constexpr (WT == kFP16)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "f"(0.f));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "f"(0.f));
 }
 
-// NT: column tiles of 8 tokens; RT: 16-row tiles of a CTA (MODE 1: half gate, half up); DI: ring depth in k blocks;
-// G32: groups of 32 k (two per block), else a block lies inside one group.
-template <int WT, int NT, int RT, int DI, bool G32, bool ZP, int MODE>
-__global__ void __launch_bounds__(kWarps * 32) w4_mma_kernel(const W4KernelParams p, const int static_weights) {
+constexpr int kWarps = 8, kRT = 4, kDI = 2;     // warps of a CTA, row tiles of a warp, ring depth in units
+
+// NT: column tiles of 8 tokens; RT: 16-row tiles of a warp (MODE 1: half gate, half up); DI: ring depth in units of 128 k;
+// G: group size; ZP: zero points given.
+template <int WT, int NT, int RT, int DI, int G, bool ZP, int MODE>
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) w4_mma_kernel(const W4KernelParams p, const int static_weights) {
     extern __shared__ __align__(128) uint8_t smem[];
     using D = W4Decode<WT>;
+    constexpr int RO = MODE == 1 ? RT / 2 : RT;          // output tiles of a warp
+    constexpr int NG = 128 / G, SG = G / 16;             // groups of a unit, 16-k steps of a group
+    constexpr uint32_t kSlot = RT * 2 * kW4BlockBytes;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, t = lane & 3;
     const int rank = blockIdx.y, SK = gridDim.y;
-    constexpr int RO = MODE == 1 ? RT / 2 : RT;          // output tiles of this CTA
-    const int tile0 = blockIdx.x * RO;
+    const int WR = p.row_warps, WK = kWarps / WR, wr = warp / WK, wk = warp - wr * WK;
+    const int tile0 = blockIdx.x * RO * WR;
 
-    if constexpr (MODE != 0) {
-        pdl_wait();                                      // the work list comes from the kernel before
-        pdl_launch_dependents();
-    } else if (!static_weights) {
+    const bool early = MODE == 0 && static_weights;      // weights may be read before the kernel in front has finished
+    if (!early) {
         pdl_wait();
         pdl_launch_dependents();
     }
@@ -69,58 +95,92 @@ __global__ void __launch_bounds__(kWarps * 32) w4_mma_kernel(const W4KernelParam
         ntok = min(NT * 8, p.n - n0);
     } else {
         const int items = p.worklist[0].x;
-        if ((int)blockIdx.z >= items) return;            // uniform over the cluster
         const int4 item = p.worklist[1 + blockIdx.z];
+        if ((int)blockIdx.z >= items) return;            // uniform over the cluster
         mat = item.x; pos0 = item.y; ntok = item.z; cpos0 = item.w;
     }
 
-    // the row tiles of this CTA; tiles past the end repeat the last one and are not stored
-    const uint8_t* wbase[RT];
-    size_t sbase[RT];
+    // tile j of row warp w; tiles past the end repeat the last one and are not stored
+    auto tile_of = [&](int w, int j) {
+        const int tile = min(tile0 + w * RO + (MODE == 1 ? j % RO : j), p.out_tiles - 1);
+        return MODE == 1 && j >= RO ? tile + p.out_tiles : tile;
+    };
+    const int units = (p.kc + 1) >> 1;                   // two blocks (128 k) each; the last one of an odd number is half
+    const int ub = (int)((long long)units * rank / SK), ue = (int)((long long)units * (rank + 1) / SK);
+    const size_t tile_bytes = (size_t)p.kc * kW4BlockBytes;
+    const uint8_t* wnext[RT];                            // the unit that is fetched next
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {
-        int tile = min(tile0 + (MODE == 1 ? i % RO : i), p.out_tiles - 1);
-        if (MODE == 1 && i >= RO) tile += p.out_tiles;
-        const size_t at = (size_t)mat * p.mat_tiles + tile;
-        wbase[i] = p.q + at * p.kc * kW4BlockBytes + lane * 16;
-        sbase[i] = at * p.groups * 8 + r;
-    }
-    const int cb = (int)((long long)p.kc * rank / SK), ce = (int)((long long)p.kc * (rank + 1) / SK);
-    const int nit = (ce - cb - warp + kWarps - 1) / kWarps;
-    const uint32_t ring = smem_u32(smem) + warp * (DI * RT * kW4BlockBytes) + lane * 16;
+    for (int i = 0; i < RT; ++i)
+        wnext[i] = p.q + ((size_t)mat * p.mat_tiles + tile_of(wr, i)) * tile_bytes + (size_t)(ub + wk) * 1024 + lane * 16;
+    const uint32_t smem0 = smem_u32(smem);
+    const uint32_t ring0 = smem0 + warp * (DI * kSlot) + lane * 16, ring1 = ring0 + DI * kSlot;
     const uint64_t pol = l2_policy_evict_first();
 
-    auto fetch = [&](int i) {
-        if (i < nit) {
-            const size_t off = (size_t)(cb + warp + i * kWarps) * kW4BlockBytes;
-            const uint32_t slot = ring + (i % DI) * (RT * kW4BlockBytes);
+    int fu = ub + wk;
+    uint32_t put = ring0, get = ring0;
+    auto fetch = [&]() {
+        if (fu < ue) {
+            const bool second = fu * 2 + 1 < p.kc;
 #pragma unroll
-            for (int j = 0; j < RT; ++j) cp_async16_hint(slot + j * kW4BlockBytes, wbase[j] + off, pol);
+            for (int j = 0; j < RT; ++j) {
+                cp_async16_hint(put + j * 1024, wnext[j], pol);
+                if (second) cp_async16_hint(put + j * 1024 + kW4BlockBytes, wnext[j] + kW4BlockBytes, pol);
+                wnext[j] += WK * 1024;
+            }
+            put = put + kSlot == ring1 ? ring0 : put + kSlot;
+            fu += WK;
         }
         cp_async_commit();                               // an empty group keeps the count
     };
-#pragma unroll
-    for (int i = 0; i < DI; ++i) fetch(i);
-    if constexpr (MODE == 0) {
-        if (static_weights) {
-            pdl_launch_dependents();
-            pdl_wait();
-        }
-    }
 
-    const uint8_t* xrow[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const int c = nt * 8 + r;
-        xrow[nt] = nullptr;
-        if (c < ntok) {
-            long long row;
-            if constexpr (MODE == 0) row = n0 + c;
-            else if constexpr (MODE == 1) row = p.sorted[pos0 + c] / p.topk;
-            else row = cpos0 + c;
-            xrow[nt] = reinterpret_cast<const uint8_t*>(p.X) + row * (2LL * p.k) + 8 * t;
+    // staging area: activations [token][pitch], scales [row tile][group][8][2], zero points likewise.  Tokens behind the
+    // last one, k behind the end, and the groups there are zeros: the loop below needs no case for them.
+    const uint32_t xs = smem0 + kWarps * DI * kSlot;
+    const uint32_t pitch = (uint32_t)p.seg_units * 256 + 32;     // 32 bytes off a multiple of 128: no bank conflicts
+    const int sg = p.seg_units * NG;
+    const uint32_t ss = xs + NT * 8 * pitch, zs = ss + (uint32_t)(WR * RT) * sg * 32;
+    auto stage = [&](int u0, int u1) {
+        const int k0 = u0 * 128, v = (min(u1 * 128, p.k) - k0) / 8, all = (u1 - u0) * 16;     // 16-byte pieces of a row
+        for (int i = tid; i < all * NT * 8; i += kWarps * 32) {
+            const int c = i / all, o = i - c * all;
+            const bool in = c < ntok && o < v;
+            const uint8_t* src = reinterpret_cast<const uint8_t*>(p.X);
+            if (in) {
+                long long row;
+                if constexpr (MODE == 0) row = n0 + c;
+                else if constexpr (MODE == 1) row = p.sorted[pos0 + c] / p.topk;
+                else row = cpos0 + c;
+                src += (row * p.k + k0) * 2 + o * 16;
+            }
+            cp_async16(xs + c * pitch + o * 16, src, in ? 16 : 0);
         }
+        const int g0 = u0 * NG, sv = (u1 - u0) * NG * 2;
+        for (int i = tid; i < WR * RT * sv; i += kWarps * 32) {
+            const int j = i / sv, o = i - j * sv;
+            const bool in = g0 + o / 2 < p.groups;
+            const size_t at = ((size_t)mat * p.mat_tiles + tile_of(j / RT, j % RT)) * p.groups + g0;
+            cp_async16(ss + (j * sg * 2 + o) * 16, reinterpret_cast<const uint8_t*>(p.s) + (in ? at * 32 + o * 16 : 0), in ? 16 : 0);
+            if (ZP && !(o & 1))
+                cp_async16(zs + (j * sg * 2 + o) * 8, reinterpret_cast<const uint8_t*>(p.z) + (in ? at * 16 + o * 8 : 0), in ? 16 : 0);
+        }
+    };
+
+    if (early) {
+#pragma unroll
+        for (int i = 0; i < DI; ++i) fetch();
+        pdl_launch_dependents();
+        pdl_wait();
+        stage(ub, min(ub + p.seg_units, ue));
+        cp_async_commit();
+        cp_async_wait<0>();
+    } else {
+        stage(ub, min(ub + p.seg_units, ue));
+        cp_async_commit();
+#pragma unroll
+        for (int i = 0; i < DI; ++i) fetch();
+        cp_async_wait<DI>();
     }
+    __syncthreads();
 
     float tot[RT][NT][4];
 #pragma unroll
@@ -130,61 +190,61 @@ __global__ void __launch_bounds__(kWarps * 32) w4_mma_kernel(const W4KernelParam
 #pragma unroll
             for (int e = 0; e < 4; ++e) tot[i][nt][e] = 0.f;
 
-    for (int it = 0; it < nit; ++it) {
-        const int c = cb + warp + it * kWarps;
-        const bool half_only = G32 && c * kW4BlockK + 32 >= p.k;     // k ends in the middle of the block
-        uint2 x[NT][4];
+    int u = ub + wk;
+    for (int u0 = ub; u0 < ue; u0 += p.seg_units) {
+        const int u1 = min(u0 + p.seg_units, ue);
+        if (u0 > ub) {                                   // the next segment of activations and scales
+            __syncthreads();
+            stage(u0, u1);
+            cp_async_commit();
+            cp_async_wait<0>();
+            __syncthreads();
+        }
+        uint32_t xa = xs + r * pitch + (u - u0) * 256 + 8 * t;
+        uint32_t sa = ss + (uint32_t)(wr * RT * sg + (u - u0) * NG) * 32 + 4 * r;
+        uint32_t za = zs + (uint32_t)(wr * RT * sg + (u - u0) * NG) * 16 + 2 * r;
+        for (; u < u1; u += WK) {
+            uint2 x[NT][8];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                x[nt][j] = make_uint2(0u, 0u);
-                if (xrow[nt] != nullptr && !(half_only && j >= 2)) x[nt][j] = ld_x(xrow[nt] + (size_t)c * (kW4BlockK * 2) + j * 32);
-            }
-        constexpr int NG = G32 ? 2 : 1;
-        const int g0 = G32 ? 2 * c : (c * kW4BlockK) >> p.group_shift;
-        uint32_t sc[RT][NG], zp[RT][NG];
+                for (int j = 0; j < 8; ++j) x[nt][j] = lds8(xa + nt * 8 * pitch + 32 * j);
+            cp_async_wait<DI - 1>();
 #pragma unroll
-        for (int i = 0; i < RT; ++i)
+            for (int i = 0; i < RT; ++i) {
+                const uint4 w0 = lds16(get + i * 1024), w1 = lds16(get + i * 1024 + kW4BlockBytes);
+                const uint32_t words[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                const size_t at = sbase[i] + (size_t)((G32 && g == 1 && half_only) ? g0 : g0 + g) * 8;
-                sc[i][g] = __ldg(p.s + at);
-                zp[i][g] = ZP ? (uint32_t)__ldg(p.z + at) : 0x0808u;
-            }
-        cp_async_wait<DI - 1>();
-        const uint32_t slot = ring + (it % DI) * (RT * kW4BlockBytes);
+                for (int g = 0; g < NG; ++g) {
+                    uint32_t zl, zh;
+                    D::zero(ZP ? lds2(za + (i * sg + g) * 16) : 0x0808u, zl, zh);
+                    const float2 s2 = unpack2<WT>(lds4(sa + (i * sg + g) * 32));
+                    float acc[NT][4];
 #pragma unroll
-        for (int i = 0; i < RT; ++i) {
-            const uint4 w = lds16(slot + i * kW4BlockBytes);
-            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+                    for (int j = g * SG; j < (g + 1) * SG; ++j) {
+                        uint32_t a[4];
+                        D::word(words[j], zl, zh, a);
 #pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                uint32_t zl, zh;
-                D::zero(zp[i][g], zl, zh);
-                float acc[NT][4];
-#pragma unroll
-                for (int j = g * (4 / NG); j < (g + 1) * (4 / NG); ++j) {
-                    uint32_t a[4];
-                    D::word(words[j], zl, zh, a);
+                        for (int nt = 0; nt < NT; ++nt) {
+                            if (j == g * SG) mma_first<WT>(acc[nt], a, x[nt][j]);
+                            else mma16816<WT>(acc[nt], a[0], a[1], a[2], a[3], x[nt][j].x, x[nt][j].y);
+                        }
+                    }
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        if (j == g * (4 / NG)) mma_first<WT>(acc[nt], a, x[nt][j]);
-                        else mma16816<WT>(acc[nt], a[0], a[1], a[2], a[3], x[nt][j].x, x[nt][j].y);
+                        tot[i][nt][0] = fmaf(s2.x, acc[nt][0], tot[i][nt][0]);
+                        tot[i][nt][1] = fmaf(s2.x, acc[nt][1], tot[i][nt][1]);
+                        tot[i][nt][2] = fmaf(s2.y, acc[nt][2], tot[i][nt][2]);
+                        tot[i][nt][3] = fmaf(s2.y, acc[nt][3], tot[i][nt][3]);
                     }
                 }
-                if (G32 && g == 1 && half_only) continue;
-                const float2 s2 = unpack2<WT>(sc[i][g]);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    tot[i][nt][0] = fmaf(s2.x, acc[nt][0], tot[i][nt][0]);
-                    tot[i][nt][1] = fmaf(s2.x, acc[nt][1], tot[i][nt][1]);
-                    tot[i][nt][2] = fmaf(s2.y, acc[nt][2], tot[i][nt][2]);
-                    tot[i][nt][3] = fmaf(s2.y, acc[nt][3], tot[i][nt][3]);
-                }
             }
+            get = get + kSlot == ring1 ? ring0 : get + kSlot;
+            xa += WK * 256;
+            sa += WK * NG * 32;
+            za += WK * NG * 16;
+            fetch();
         }
-        fetch(it + DI);
     }
 
     // ---- partial sums of the warps, then of the cluster ----
@@ -203,112 +263,190 @@ __global__ void __launch_bounds__(kWarps * 32) w4_mma_kernel(const W4KernelParam
             d[kTokStride + 8] = D::kFactorHigh * tot[i][nt][3];
         }
     __syncthreads();
-    auto place = [&](int i, int tok, int row) { return (i * NT * 8 + tok) * kTokStride + row; };
-    for (int e = tid; e < RT * 16 * ntok; e += kWarps * 32) {
-        const int row = e & 15, i = (e >> 4) % RT, tok = (e >> 4) / RT;
-        const int at = place(i, tok, row);
-        float v = red[at];
-#pragma unroll
-        for (int w = 1; w < kWarps; ++w) v += red[w * kPerWarp + at];
-        red[at] = v;
-    }
-    uint32_t remote[8];
-    __syncwarp();
-    if (SK > 1) {
-        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-#pragma unroll
-        for (int q = 0; q < 8; ++q)
-            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote[q]) : "r"(smem_u32(smem)), "r"(q < SK ? q : 0));
-    } else {
-        __syncthreads();
-    }
-    auto total = [&](int at) {
-        if (SK == 1) return red[at];
-        float v = 0.f;
-#pragma unroll
-        for (int q = 0; q < 8; ++q)
-            if (q < SK) {
-                float u;
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(u) : "r"(remote[q] + 4u * at) : "memory");
-                v += u;
-            }
+    // four rows at a time: the sums of row warp w's tile i, token tok, rows 4 q .. of 16
+    auto place = [&](int w, int i, int tok, int q) { return w * WK * kPerWarp + (i * NT * 8 + tok) * kTokStride + 4 * q; };
+    auto add = [](float4& v, float4 o) { v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w; };
+    auto warps_sum = [&](int at) {
+        float4 v = *reinterpret_cast<const float4*>(red + at);
+        for (int q = 1; q < WK; ++q) add(v, *reinterpret_cast<const float4*>(red + q * kPerWarp + at));
         return v;
     };
-    const int outs = RO * 16 * ntok;
+    if (SK > 1) {
+        if (WK > 1) {
+            for (int e = tid; e < WR * RT * 4 * ntok; e += kWarps * 32) {
+                const int q = e & 3, i = (e >> 2) % RT, rest = (e >> 2) / RT, w = rest % WR, tok = rest / WR;
+                const int at = place(w, i, tok, q);
+                *reinterpret_cast<float4*>(red + at) = warps_sum(at);
+            }
+        }
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+    auto total = [&](int at) {
+        if (SK == 1) return warps_sum(at);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int q = 0; q < SK; ++q) {
+            uint32_t a;
+            float4 o;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem0 + 4u * at), "r"(q));
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(o.x), "=f"(o.y), "=f"(o.z), "=f"(o.w) : "r"(a) : "memory");
+            add(v, o);
+        }
+        return v;
+    };
+    const int outs = WR * RO * 4 * ntok;
+    const size_t ld = (size_t)p.out_tiles * 16;
     for (int e = outs * rank / SK + tid; e < outs * (rank + 1) / SK; e += kWarps * 32) {
-        const int row16 = e & 15, i = (e >> 4) % RO, tok = (e >> 4) / RO;
-        if (tile0 + i >= p.out_tiles) continue;
-        const int row = (tile0 + i) * 16 + row16;
-        const size_t ld = (size_t)p.out_tiles * 16;
-        const float v = total(place(i, tok, row16));
+        const int q = e & 3, i = (e >> 2) % RO, rest = (e >> 2) / RO, w = rest % WR, tok = rest / WR;
+        const int tile = tile0 + w * RO + i;
+        if (tile >= p.out_tiles) continue;
+        const int row = tile * 16 + 4 * q;
+        const float4 v = total(place(w, i, tok, q));
         if constexpr (MODE == 0) {
-            const float b = p.bias ? load_scalar16<WT>(p.bias, row) : 0.f;
-            store16<WT>(p.C, (size_t)(n0 + tok) * ld + row, fmaf(p.alpha, v, b));
+            float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (p.bias) b = make_float4(load_scalar16<WT>(p.bias, row), load_scalar16<WT>(p.bias, row + 1), load_scalar16<WT>(p.bias, row + 2), load_scalar16<WT>(p.bias, row + 3));
+            uint2 o;
+            o.x = pack2<WT>(fmaf(p.alpha, v.x, b.x), fmaf(p.alpha, v.y, b.y));
+            o.y = pack2<WT>(fmaf(p.alpha, v.z, b.z), fmaf(p.alpha, v.w, b.w));
+            *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.C) + (size_t)(n0 + tok) * ld + row) = o;
         } else if constexpr (MODE == 1) {
-            const float up = total(place(i + RO, tok, row16));
-            store16<WT>(p.C, (size_t)(cpos0 + tok) * ld + row, v / (1.f + __expf(-v)) * up);
+            const float4 up = total(place(w, i + RO, tok, q));
+            auto act = [](float g, float h) { return g / (1.f + __expf(-g)) * h; };
+            uint2 o;
+            o.x = pack2<WT>(act(v.x, up.x), act(v.y, up.y));
+            o.y = pack2<WT>(act(v.z, up.z), act(v.w, up.w));
+            *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.C) + (size_t)(cpos0 + tok) * ld + row) = o;
         } else {
             const int slot = p.sorted[pos0 + tok];
-            reinterpret_cast<float*>(p.C)[(size_t)slot * ld + row] = load_scalar16<WT>(p.topk_weights, slot) * v;
+            const float f = load_scalar16<WT>(p.topk_weights, slot);
+            *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.C) + (size_t)slot * ld + row) = make_float4(f * v.x, f * v.y, f * v.z, f * v.w);
         }
     }
-    __syncwarp();
-    if (SK > 1)     // nobody leaves while its shared memory may still be read
+    if (SK > 1) {                                        // nobody leaves while its shared memory may still be read
+        __syncwarp();
         asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
 }
 
-template <int WT, int NT, int RT, int DI, int MODE>
-const void* pick(bool g32, bool zp) {
-    if (g32) return zp ? reinterpret_cast<const void*>(w4_mma_kernel<WT, NT, RT, DI, true, true, MODE>)
-                       : reinterpret_cast<const void*>(w4_mma_kernel<WT, NT, RT, DI, true, false, MODE>);
-    return zp ? reinterpret_cast<const void*>(w4_mma_kernel<WT, NT, RT, DI, false, true, MODE>)
-              : reinterpret_cast<const void*>(w4_mma_kernel<WT, NT, RT, DI, false, false, MODE>);
+template <int WT, int NT, int MODE>
+const void* pick(int group, bool zp) {
+    if (group == 128) return zp ? reinterpret_cast<const void*>(w4_mma_kernel<WT, NT, kRT, kDI, 128, true, MODE>)
+                                : reinterpret_cast<const void*>(w4_mma_kernel<WT, NT, kRT, kDI, 128, false, MODE>);
+    if (group == 64) return zp ? reinterpret_cast<const void*>(w4_mma_kernel<WT, NT, kRT, kDI, 64, true, MODE>)
+                               : reinterpret_cast<const void*>(w4_mma_kernel<WT, NT, kRT, kDI, 64, false, MODE>);
+    return zp ? reinterpret_cast<const void*>(w4_mma_kernel<WT, NT, kRT, kDI, 32, true, MODE>)
+              : reinterpret_cast<const void*>(w4_mma_kernel<WT, NT, kRT, kDI, 32, false, MODE>);
 }
-template <int NT, int RT, int DI, int MODE>
-const void* pick(int wt, bool g32, bool zp) {
-    return wt == kFP16 ? pick<kFP16, NT, RT, DI, MODE>(g32, zp) : pick<kBF16, NT, RT, DI, MODE>(g32, zp);
+template <int NT>
+const void* pick(int mode, int wt, int group, bool zp) {
+    if (wt == kFP16)
+        return mode == 0 ? pick<kFP16, NT, 0>(group, zp) : (mode == 1 ? pick<kFP16, NT, 1>(group, zp) : pick<kFP16, NT, 2>(group, zp));
+    return mode == 0 ? pick<kBF16, NT, 0>(group, zp) : (mode == 1 ? pick<kBF16, NT, 1>(group, zp) : pick<kBF16, NT, 2>(group, zp));
+}
+
+// Clusters of sk CTAs that the device holds at once.  A cluster sits inside one group of SMs, so for sk > 2 this is less
+// than the SMs suggest, and a launch that exceeds it by one cluster takes another round.
+int active_clusters(const void* kern, size_t smem, int sk, int resident) {
+    if (sk == 1) return resident * sm_count();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1, (unsigned)sk);
+    cfg.blockDim = dim3(kWarps * 32);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1;
+    attr[0].val.clusterDim.y = (unsigned)sk;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) n = 0;
+    cudaGetLastError();
+    return n;
+}
+
+struct Plan {
+    int wr, sk, seg;
+    size_t smem;                // launch size, 0 = the kernel cannot run here
+};
+
+// Row warps, cluster size and staging of a launch, by an estimate of its time that knows four things: a CTA costs 2.5 us
+// to start, stage and reduce; a CTA alone on an SM takes 0.95 us for an iteration of its warps (32 KB of weights) with 8
+// tokens, 2.0 with 16; several on an SM share the memory at 0.87 and 1.1 us per CTA; and rounds are whole.  (Fitted to
+// sweeps over 4096 x 4096 .. 28672 x 8192 and the expert shapes; the best and the chosen split differ by at most 8 % there.)
+Plan make_plan(const void* kern, int mode, int nt, int group, bool zp, int tiles, int units, int items) {
+    Plan best{1, 1, 1, 0};
+    double best_us = 1e30;
+    const size_t ring = (size_t)kWarps * kDI * kRT * 1024;
+    for (int wr = 1; wr <= kWarps; wr *= 2)
+        for (int sk = 1; sk <= 8 && sk <= units; ++sk) {
+            const int ro = (mode == 1 ? kRT / 2 : kRT) * wr, wk = kWarps / wr;
+            if (wr > 1 && ro / 2 >= tiles) continue;                    // half of the row warps would have nothing to do
+            auto staged = [&](int n) { return (size_t)nt * 8 * (n * 256 + 32) + (size_t)wr * kRT * n * (128 / group) * (zp ? 48 : 32); };
+            // a segment: the CTA's whole k range where it fits beside the ring, else as many units as do
+            int seg = (units + sk - 1) / sk;
+            while (ring + staged(seg) > 200 * 1024) seg = (seg + 1) / 2;
+            const size_t smem = std::max(ring + staged(seg), (size_t)kWarps * kRT * nt * 8 * kTokStride * 4);
+            int resident = 0;
+            const size_t launch_smem = umma::prepare_kernel(kern, kWarps * 32, smem, 0, false, &resident);
+            if (launch_smem == 0) continue;
+            const int room = active_clusters(kern, launch_smem, sk, resident);
+            if (room < 1) continue;
+            const int per_rank = (units + sk - 1) / sk;
+            const double clusters = (double)((tiles + ro - 1) / ro) * items, iters = (per_rank + wk - 1) / wk;
+            const double rounds = std::ceil(clusters / room), share = std::min<double>(resident, std::ceil(clusters * sk / sm_count()));
+            const double iter_us = nt == 1 ? std::max(0.95, 0.87 * share) : std::max(2.0, 1.1 * share);
+            const double us = rounds * (2.5 * ((per_rank + seg - 1) / seg) + iters * iter_us) + (sk > 1 ? 0.5 : 0.0);
+            if (us < best_us) {
+                best_us = us;
+                best = Plan{wr, sk, seg, launch_smem};
+            }
+        }
+    return best;
+}
+
+Plan cached_plan(const void* kern, int mode, int nt, int group, bool zp, int tiles, int units, int items) {
+    static std::mutex mu;
+    static std::map<std::array<long long, 6>, Plan> known;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return Plan{1, 1, 1, 0};
+    const std::array<long long, 6> key{(long long)(uintptr_t)kern, dev, tiles, units, items, 0};
+    std::lock_guard<std::mutex> lock(mu);
+    auto it = known.find(key);
+    if (it != known.end()) return it->second;
+    if (known.size() > 4096) known.clear();              // a server sees a few hundred shapes
+    return known[key] = make_plan(kern, mode, nt, group, zp, tiles, units, items);
 }
 
 }  // namespace
 
-int launch_w4_mma(int mode, int wt, W4KernelParams p, const W4Weights& w, int token_blocks, int nt, int sk, cudaStream_t s) {
-    constexpr int RT = 2, DI = 4;
-    const bool g32 = w.group == 32, zp = w.z != nullptr;
-    const void* kern = nullptr;
-    if (mode == 0) kern = nt == 1 ? pick<1, RT, DI, 0>(wt, g32, zp) : pick<2, RT, DI, 0>(wt, g32, zp);
-    else if (mode == 1) kern = nt == 1 ? pick<1, RT, DI, 1>(wt, g32, zp) : pick<2, RT, DI, 1>(wt, g32, zp);
-    else kern = nt == 1 ? pick<1, RT, DI, 2>(wt, g32, zp) : pick<2, RT, DI, 2>(wt, g32, zp);
-    const int ro = mode == 1 ? RT / 2 : RT;
-    const size_t smem = std::max((size_t)kWarps * DI * RT * kW4BlockBytes, (size_t)kWarps * RT * nt * 8 * kTokStride * 4);
-    const size_t launch_smem = umma::prepare_kernel(kern, kWarps * 32, smem, 0);
-    if (launch_smem == 0) return fail(kCudaError, "w4: the streaming kernel cannot be launched on this device");
-    if (token_blocks > 65535) return fail(kUnsupported, "w4: %d token blocks exceed one launch", token_blocks);
+int launch_w4_mma(int mode, int wt, W4KernelParams p, const W4Weights& w, int items, int likely_items, int nt, cudaStream_t s) {
+    const bool zp = w.z != nullptr;
+    p.kc = (p.k + kW4BlockK - 1) / kW4BlockK;
+    p.groups = p.k / w.group;
     p.q = w.q;
     p.s = reinterpret_cast<const uint32_t*>(w.s);
     p.z = reinterpret_cast<const uint16_t*>(w.z);
-    p.kc = (p.k + kW4BlockK - 1) / kW4BlockK;
-    p.groups = p.k / w.group;
-    p.group_shift = w.group == 128 ? 7 : (w.group == 64 ? 6 : 5);
+    if (items > 65535) return fail(kUnsupported, "w4: %d work items exceed one launch", items);
+    const void* kern = nt == 1 ? pick<1>(mode, wt, w.group, zp) : pick<2>(mode, wt, w.group, zp);
+    const Plan q = cached_plan(kern, mode, nt, w.group, zp, p.out_tiles, (p.kc + 1) / 2, likely_items);
+    if (q.smem == 0) return fail(kCudaError, "w4: the streaming kernel cannot be launched on this device");
+    p.seg_units = q.seg;
+    p.row_warps = q.wr;
+    const int ro = (mode == 1 ? kRT / 2 : kRT) * q.wr;
     int static_weights = option(kOptStaticWeights);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((p.out_tiles + ro - 1) / ro), (unsigned)sk, (unsigned)token_blocks);
+    cfg.gridDim = dim3((unsigned)((p.out_tiles + ro - 1) / ro), (unsigned)q.sk, (unsigned)items);
     cfg.blockDim = dim3(kWarps * 32);
-    cfg.dynamicSmemBytes = launch_smem;
+    cfg.dynamicSmemBytes = q.smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
     cfg.attrs = attr;
-    cfg.numAttrs = launch_attrs(attr, sk);
+    cfg.numAttrs = launch_attrs(attr, q.sk);
     void* args[2] = {&p, &static_weights};
     const cudaError_t e = cudaLaunchKernelExC(&cfg, kern, args);
     if (e != cudaSuccess) return fail(kCudaError, "w4 launch: %s", cudaGetErrorString(e));
     return kOk;
-}
-
-// k parts: enough warps for the whole chip to have its loads in flight at once, at least two k blocks per warp.
-int w4_mma_split(long long row_ctas, int kc) {
-    int sk = 1;
-    while (sk < 8 && row_ctas * sk < 3LL * sm_count() && kc / (kWarps * sk * 2) >= 2) sk *= 2;
-    return sk;
 }
 
 }  // namespace mlk
