@@ -15,9 +15,9 @@ from typing import Optional
 
 import torch
 
-from ._lib import check, lib
-from .ext import _chk, _cuda_contig, _ptr, _stream
-from .w4 import _on, _same_device
+from ._lib import lib
+from .ext import _chk, _cuda_contig, _ptr
+from .w4 import _launch, _same_device
 
 __all__ = ["router_balance_loss", "expert_counts"]
 
@@ -33,6 +33,16 @@ def _mask_ptr(mask: Optional[torch.Tensor], T: int):
 
 
 def _checked(x, ids, score_fun, mask, cu):
+    """Like the other operators' checks: the first test is the whole of it, the rest finds the message."""
+    d, xs, s = x.get_device(), x.shape, ids.shape
+    if (x.is_cuda and ids.get_device() == d and x.is_contiguous() and ids.is_contiguous() and x.dtype in _CODES
+            and ids.dtype is torch.int32 and len(xs) == 2 and len(s) == 2 and xs[1] > 0 and s[0] == xs[0] and s[1] > 0
+            and score_fun in (0, 1)
+            and (mask is None or (mask.get_device() == d and mask.is_contiguous() and mask.shape == xs[:1]
+                                  and (mask.dtype is torch.bool or mask.dtype is torch.uint8)))
+            and (cu is None or (cu.get_device() == d and cu.is_contiguous() and cu.dtype is torch.int32 and cu.dim() == 1
+                                and cu.shape[0] >= 2))):
+        return
     _cuda_contig(x, "gating_output")
     _cuda_contig(ids, "experts_ids")
     _chk(x.dtype in _CODES, "gating_output must be bfloat16, float16 or float32")
@@ -45,22 +55,23 @@ def _checked(x, ids, score_fun, mask, cu):
         _cuda_contig(cu, "cu_seqlens")
         _chk(cu.dtype == torch.int32 and cu.dim() == 1 and cu.numel() >= 2, "cu_seqlens must be int32 [sequences + 1]")
     _same_device(x, (ids, "experts_ids"), (mask, "token_mask"), (cu, "cu_seqlens"))
+    raise RuntimeError("router_balance_loss: bad arguments")
 
 
 def _loss(x, ids, score_fun, coef, mask, cu, want_grad: bool):
-    """(loss, counts, d loss / d p, gradient or None), on the current stream."""
+    """(loss, counts, d loss / d p behind the workspace's start, gradient or None), on the current stream."""
     T, E = x.shape
-    B = 1 if cu is None else cu.numel() - 1
-    loss = torch.empty((), dtype=torch.float32, device=x.device)
-    counts = torch.empty(E, dtype=torch.int32, device=x.device)
-    dprob = torch.empty((B, E), dtype=torch.float32, device=x.device)
+    B = 1 if cu is None else cu.shape[0] - 1
+    loss = x.new_empty((), dtype=torch.float32)
+    counts = x.new_empty((E,), dtype=torch.int32)
     grad = torch.empty_like(x) if want_grad else None
-    with _on(x):
-        ws = torch.empty(lib.mlk_router_balance_workspace_bytes(T, E, B), dtype=torch.uint8, device=x.device)
-        check(lib.mlk_router_balance_loss(x.data_ptr(), ids.data_ptr(), _ptr(mask), _ptr(cu), T, E, ids.size(1), B, score_fun,
-                                          coef, _CODES[x.dtype], loss.data_ptr(), counts.data_ptr(), dprob.data_ptr(),
-                                          _ptr(grad), ws.data_ptr(), ws.numel(), _stream(x)))
-    return loss, counts, dprob, grad
+    head = (4 * B * E + 255) // 256 * 256          # d loss / d p [B, E] comes first: the backward pass reads it again
+    nbytes = lib.mlk_router_balance_workspace_bytes(T, E, B)
+    ws = x.new_empty((head + nbytes,), dtype=torch.uint8)
+    at = ws.data_ptr()
+    _launch(x.get_device(), lib.mlk_router_balance_loss, x.data_ptr(), ids.data_ptr(), _ptr(mask), _ptr(cu), T, E, ids.shape[1], B,
+            score_fun, coef, _CODES[x.dtype], loss.data_ptr(), counts.data_ptr(), at, _ptr(grad), at + head, nbytes)
+    return loss, counts, ws, grad
 
 
 class _BalanceLoss(torch.autograd.Function):
@@ -77,11 +88,9 @@ class _BalanceLoss(torch.autograd.Function):
     def backward(ctx, grad_loss, _):
         x, dprob, mask, cu = ctx.saved_tensors
         grad = torch.empty_like(x)
-        grad_loss = grad_loss.to(torch.float32)
-        with _on(x):
-            check(lib.mlk_router_balance_grad(x.data_ptr(), _ptr(mask), _ptr(cu), x.size(0), x.size(1), dprob.size(0),
-                                              ctx.score_fun, _CODES[x.dtype], dprob.data_ptr(), grad_loss.data_ptr(),
-                                              grad.data_ptr(), _stream(x)))
+        _launch(x.get_device(), lib.mlk_router_balance_grad, x.data_ptr(), _ptr(mask), _ptr(cu), x.shape[0], x.shape[1],
+                1 if cu is None else cu.shape[0] - 1, ctx.score_fun, _CODES[x.dtype], dprob.data_ptr(), grad_loss.data_ptr(),
+                grad.data_ptr())
         return grad, None, None, None, None, None
 
 
@@ -114,7 +123,6 @@ def expert_counts(experts_ids: torch.Tensor, num_experts: int, token_mask: Optio
     T, topk = experts_ids.shape
     mask = _mask_ptr(token_mask, T)
     _same_device(experts_ids, (token_mask, "token_mask"))
-    counts = torch.empty(num_experts, dtype=torch.int32, device=experts_ids.device)
-    with _on(experts_ids):
-        check(lib.mlk_expert_counts(experts_ids.data_ptr(), mask, T, topk, num_experts, counts.data_ptr(), _stream(experts_ids)))
+    counts = experts_ids.new_empty((num_experts,))
+    _launch(experts_ids.get_device(), lib.mlk_expert_counts, experts_ids.data_ptr(), mask, T, topk, num_experts, counts.data_ptr())
     return counts

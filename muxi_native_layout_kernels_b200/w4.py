@@ -16,23 +16,37 @@ stream of the tensors' device; no op synchronises, and every one can be captured
 """
 from __future__ import annotations
 
-from contextlib import nullcontext
 from typing import Optional
 
 import torch
 
 from ._lib import check, lib
-from .ext import _act_code, _bias_ptr, _chk, _cuda_contig, _map_args, _ptr, _status_ptr, _stream
+from .ext import _SYNC_BUFFERS, _bias_ptr, _chk, _cuda_contig, _map_args, _ptr, _status_ptr
 
 __all__ = ["layoutA_w4", "layoutA_w4_inverse", "layoutA_w4_groups", "gemv_layoutA_w4", "gemm_layoutA_w4",
            "fused_experts_compute_w4"]
 
 _GROUPS = (32, 64, 128)
+_CODES = {torch.bfloat16: 0, torch.float16: 1}
+_device_of_thread = torch._C._cuda_getDevice
+_stream_of = torch._C._cuda_getCurrentRawStream
 
 
-def _on(t: torch.Tensor):
-    """The tensors' device current for the launch (a no-op where it already is)."""
-    return nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+def _launch(device: int, call, *args) -> None:
+    """``call(*args, stream)`` with the tensors' device current and its current stream."""
+    if _device_of_thread() == device:
+        status = call(*args, _stream_of(device))
+    else:
+        with torch.cuda.device(device):
+            status = call(*args, _stream_of(device))
+    if status:
+        check(status)
+
+
+def _status(device: int, like: torch.Tensor) -> int:
+    """Device address of the sticky status word of the current stream."""
+    bufs = _SYNC_BUFFERS.get((device, _stream_of(device)))
+    return _status_ptr(like) if bufs is None else bufs[1].data_ptr()
 
 
 def _same_device(like: torch.Tensor, *named) -> None:
@@ -51,8 +65,7 @@ def layoutA_w4(W: torch.Tensor) -> torch.Tensor:
     _chk(m % 16 == 0 and k % 32 == 0 and k > 0, "layoutA_w4 needs m % 16 == 0 and k % 32 == 0")
     out = torch.empty(W.shape[:-2] + (m // 16, (k + 63) // 64, 32, 16), dtype=torch.uint8, device=W.device)
     rows = m * (W.shape[0] if W.dim() == 3 else 1)
-    with _on(W):
-        check(lib.mlk_layoutA_w4(W.data_ptr(), out.data_ptr(), rows, k, 0, _stream(W)))
+    _launch(W.get_device(), lib.mlk_layoutA_w4, W.data_ptr(), out.data_ptr(), rows, k, 0)
     return out
 
 
@@ -62,8 +75,7 @@ def layoutA_w4_inverse(A: torch.Tensor, k: int) -> torch.Tensor:
     R, kc = _packed_dims(A, "A")
     _chk(k > 0 and k % 32 == 0 and (k + 63) // 64 == kc, "k does not match the packed weights")
     out = torch.empty(A.shape[:-4] + (R * 16, k // 2), dtype=torch.uint8, device=A.device)
-    with _on(A):
-        check(lib.mlk_layoutA_w4(A.data_ptr(), out.data_ptr(), out.numel() // (k // 2), k, 1, _stream(A)))
+    _launch(A.get_device(), lib.mlk_layoutA_w4, A.data_ptr(), out.data_ptr(), out.numel() // (k // 2), k, 1)
     return out
 
 
@@ -77,24 +89,36 @@ def layoutA_w4_groups(values: torch.Tensor) -> torch.Tensor:
     _chk(m % 16 == 0 and G > 0, "layoutA_w4_groups needs m % 16 == 0 and at least one group")
     out = torch.empty(values.shape[:-2] + (m // 16, G, 8, 2), dtype=values.dtype, device=values.device)
     rows = m * (values.shape[0] if values.dim() == 3 else 1)
-    with _on(values):
-        check(lib.mlk_layoutA_w4_groups(values.data_ptr(), out.data_ptr(), rows, G, values.element_size(), _stream(values)))
+    _launch(values.get_device(), lib.mlk_layoutA_w4_groups, values.data_ptr(), out.data_ptr(), rows, G, values.element_size())
     return out
 
 
-def _packed_dims(A: torch.Tensor, name: str, lead: int = -1):
+def _packed_dims(A: torch.Tensor, name: str):
     _chk(A.dtype == torch.uint8, f"{name} must be uint8 (packed by layoutA_w4)")
-    _chk(A.dim() - 4 in ((0, 1) if lead < 0 else (lead,)), f"{name} must be [{'E, ' if lead == 1 else ''}m/16, ceil(k/64), 32, 16]")
+    _chk(A.dim() in (4, 5), f"{name} must be [m/16, ceil(k/64), 32, 16], or that behind an expert dimension")
     _chk(A.size(-2) == 32 and A.size(-1) == 16, f"{name}'s trailing dims must be (32, 16)")
     return A.size(-4), A.size(-3)
 
 
 def _group(A, scales, zeros, x, k: int, name: str) -> int:
-    """Group size told by the scales' shape, after checking all that belongs to one weight tensor against it."""
+    """Group size told by the scales' shape, after checking all that belongs to one weight tensor against it.  The first
+    test is the whole of it; what follows only finds the message (formatting it costs more than a small launch)."""
+    a, s = A.shape, scales.shape
+    d = x.get_device()
+    lead = len(a) - 4
+    if lead in (0, 1) and len(s) == lead + 4:
+        G = s[lead + 1]
+        if (A.get_device() == d and scales.get_device() == d and A.dtype is torch.uint8 and scales.dtype is x.dtype
+                and A.is_contiguous() and scales.is_contiguous() and a[lead + 2] == 32 and a[lead + 3] == 16
+                and s[lead + 2] == 8 and s[lead + 3] == 2 and s[:lead + 1] == a[:lead + 1] and a[lead + 1] == (k + 63) // 64
+                and G > 0 and k % G == 0 and k // G in _GROUPS
+                and (zeros is None or (zeros.get_device() == d and zeros.dtype is torch.uint8 and zeros.shape == s
+                                       and zeros.is_contiguous()))):
+            return k // G
     _cuda_contig(A, name)
     _cuda_contig(scales, f"{name} scales")
+    R, kc = _packed_dims(A, name)
     lead = A.shape[:-4]
-    R, kc = _packed_dims(A, name, len(lead))
     _chk(scales.dtype == x.dtype, f"{name} scales must have the activation data type")
     _chk(scales.dim() == len(lead) + 4 and tuple(scales.shape[-2:]) == (8, 2) and scales.shape[:len(lead)] == lead and
          scales.size(-4) == R, f"{name} scales must be [{'E, ' if lead else ''}m/16, k/group, 8, 2] (from layoutA_w4_groups)")
@@ -105,7 +129,7 @@ def _group(A, scales, zeros, x, k: int, name: str) -> int:
         _cuda_contig(zeros, f"{name} zeros")
         _chk(zeros.dtype == torch.uint8 and zeros.shape == scales.shape, f"{name} zeros must be uint8 in the shape of the scales")
     _same_device(x, (A, name), (scales, f"{name} scales"), (zeros, f"{name} zeros"))
-    return k // G
+    raise RuntimeError(f"{name}: weights, scales and zeros do not belong together")
 
 
 def gemm_layoutA_w4(A, scales, B, alpha: float = 1, beta: float = 0, zeros=None, bias=None):
@@ -116,16 +140,19 @@ def gemm_layoutA_w4(A, scales, B, alpha: float = 1, beta: float = 0, zeros=None,
     _chk(B.is_cuda, "B must be a CUDA tensor")
     _chk(B.is_contiguous(), "B must be contiguous")
     _chk(B.dim() == 2, "B must be a 2D tensor")
-    code = _act_code(B)
+    code = _CODES.get(B.dtype)
+    _chk(code is not None, "Unsupported data type")
+    _chk(A.dim() == 4, "A must be [m/16, ceil(k/64), 32, 16]")
     n, k = B.shape
-    R, _ = _packed_dims(A, "A", 0)
     group = _group(A, scales, zeros, B, k, "A")
-    m = R * 16
-    _same_device(B, (bias, "bias"))
-    C = torch.empty((n, m), dtype=B.dtype, device=B.device)
-    with _on(B):
-        check(lib.mlk_gemm_layoutA_w4(A.data_ptr(), scales.data_ptr(), _ptr(zeros), group, B.data_ptr(), C.data_ptr(), m, n, k,
-                                      code, alpha, _bias_ptr(bias, B, m), _status_ptr(B), _stream(B)))
+    m = A.shape[0] * 16
+    if bias is not None:
+        _same_device(B, (bias, "bias"))
+        bias = _bias_ptr(bias, B, m)
+    C = B.new_empty((n, m))
+    d = B.get_device()
+    _launch(d, lib.mlk_gemm_layoutA_w4, A.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(), group,
+            B.data_ptr(), C.data_ptr(), m, n, k, code, alpha, bias, _status(d, B))
     return C
 
 
@@ -146,37 +173,39 @@ def fused_experts_compute_w4(w1, w1_scales, w2, w2_scales, activations, topk_ids
     un-rounded sums; ``out`` receives the result (every element is written).  A token's experts are added in
     slot order in fp32 with one rounding."""
     x = activations
-    _cuda_contig(x, "activations")
+    _chk(x.is_cuda and x.is_contiguous(), "activations must be a contiguous CUDA tensor")
     _chk(x.dim() == 2, "activations must be [T, H]")
-    code = _act_code(x)
+    code = _CODES.get(x.dtype)
+    _chk(code is not None, "Unsupported data type")
     T, H = x.shape
-    _packed_dims(w1, "w1", 1)
-    _packed_dims(w2, "w2", 1)
-    E, I = w1.size(0), w1.size(1) * 8
-    _chk(w1.size(1) % 2 == 0 and w2.size(0) == E and w2.size(1) * 16 == H and E > 0, "w1 must hold [E, 2I, H] and w2 [E, H, I]")
+    _chk(w1.dim() == 5 and w2.dim() == 5, "w1 and w2 must be [E, rows/16, ceil(k/64), 32, 16]")
+    s1, s2 = w1.shape, w2.shape
+    E, I = s1[0], s1[1] * 8
+    _chk(s1[1] % 2 == 0 and s2[0] == E and s2[1] * 16 == H and E > 0, "w1 must hold [E, 2I, H] and w2 [E, H, I]")
     g1 = _group(w1, w1_scales, w1_zeros, x, H, "w1")
     g2 = _group(w2, w2_scales, w2_zeros, x, I, "w2")
-    _cuda_contig(topk_ids, "topk_ids")
-    _cuda_contig(topk_weights, "topk_weights")
-    _chk(topk_ids.dtype == torch.int32 and topk_ids.dim() == 2 and topk_ids.size(0) == T and topk_ids.size(1) > 0,
-         "topk_ids must be int32 [T, topk]")
-    _chk(topk_weights.dtype == x.dtype and topk_weights.shape == topk_ids.shape,
-         "topk_weights must be [T, topk] in the activation data type")
-    _same_device(x, (topk_ids, "topk_ids"), (topk_weights, "topk_weights"), (experts_map, "experts_map"), (out, "out"))
-    mp, ml = _map_args(experts_map)
+    d = x.get_device()
+    ids = topk_ids.shape
+    _chk(topk_ids.get_device() == d and topk_ids.is_contiguous() and topk_ids.dtype is torch.int32 and len(ids) == 2 and
+         ids[0] == T and ids[1] > 0, "topk_ids must be a contiguous int32 [T, topk] on the activations' device")
+    _chk(topk_weights.get_device() == d and topk_weights.is_contiguous() and topk_weights.dtype is x.dtype and
+         topk_weights.shape == ids, "topk_weights must be a contiguous [T, topk] in the activation data type and on its device")
+    mp, ml = None, 0
+    if experts_map is not None:
+        _same_device(x, (experts_map, "experts_map"))
+        mp, ml = _map_args(experts_map)
     dtype = x.dtype if out_dtype is None else out_dtype
-    _chk(dtype in (x.dtype, torch.float32), "out_dtype must be the activation data type or torch.float32")
+    _chk(dtype is x.dtype or dtype is torch.float32, "out_dtype must be the activation data type or torch.float32")
     if out is None:
-        out = torch.empty((T, H), dtype=dtype, device=x.device)
+        out = x.new_empty((T, H), dtype=dtype)
     else:
-        _cuda_contig(out, "out")
-        _chk(out.shape == x.shape and out.dtype == dtype, "out must be [T, H] in the result's data type")
-    topk = topk_ids.size(1)
-    with _on(x):
-        ws = torch.empty(lib.mlk_experts_w4_workspace_bytes(T, E, topk, H, I), dtype=torch.uint8, device=x.device)
-        check(lib.mlk_fused_experts_compute_w4(
-            w1.data_ptr(), w1_scales.data_ptr(), _ptr(w1_zeros), g1, w2.data_ptr(), w2_scales.data_ptr(), _ptr(w2_zeros), g2,
-            x.data_ptr(), T, E, topk, H, I, topk_ids.data_ptr(), topk_weights.data_ptr(), out.data_ptr(), code,
-            int(dtype == torch.float32 and x.dtype != torch.float32), mp, ml, ws.data_ptr(), ws.numel(), _status_ptr(x),
-            _stream(x)))
+        _chk(out.get_device() == d and out.is_contiguous() and out.shape == x.shape and out.dtype is dtype,
+             "out must be a contiguous [T, H] in the result's data type on the activations' device")
+    topk = ids[1]
+    nbytes = lib.mlk_experts_w4_workspace_bytes(T, E, topk, H, I)
+    ws = x.new_empty((nbytes,), dtype=torch.uint8)
+    _launch(d, lib.mlk_fused_experts_compute_w4, w1.data_ptr(), w1_scales.data_ptr(), _ptr(w1_zeros), g1, w2.data_ptr(),
+            w2_scales.data_ptr(), _ptr(w2_zeros), g2, x.data_ptr(), T, E, topk, H, I, topk_ids.data_ptr(),
+            topk_weights.data_ptr(), out.data_ptr(), code, int(dtype is torch.float32), mp, ml, ws.data_ptr(), nbytes,
+            _status(d, x))
     return out
