@@ -42,6 +42,7 @@ SOURCES = [
     "w4_pack.cu",
     "w4_dense.cu",
     "w4_mma.cu",
+    "w4_umma.cu",
     "w4_experts.cu",
     "selector.cpp",
 ]

@@ -1,5 +1,7 @@
 // Products of one 4-bit matrix with n tokens: argument checks and the choice of the kernel.
 #include <algorithm>
+#include <cstdio>
+#include <cstdlib>
 
 #include "w4_kernels.cuh"
 
@@ -24,11 +26,17 @@ int launch_w4_dense(const W4DenseParams& p, cudaStream_t s) {
     g.bias = p.bias;
     g.out_tiles = g.mat_tiles = p.m / 16;
     g.k = p.k;
-    const int nt = p.n <= 8 ? 1 : 2, block = 8 * nt;
     g.X = p.X;
     g.C = p.C;
     g.n = p.n;
-    const int items = (p.n + block - 1) / block;
+    int np = p.n <= 32 ? 32 : (p.n <= 64 ? 64 : (p.n <= 128 ? 128 : 256)), sk = 0, lim = 16;
+    if (const char* v = getenv("W4_U")) sscanf(v, "%d,%d,%d", &lim, &np, &sk);
+    if (p.n > lim) {
+        const int tokens = (p.n + np - 1) / np, tiles = (g.out_tiles + 7) / 8, stages = (p.k + 127) / 128;
+        if (sk == 0) { sk = 1; while (sk < 8 && np <= 128 && tiles * tokens * sk < sm_count() && stages / sk >= 4) ++sk; }
+        return launch_w4_umma(0, p.dtype, g, p.w, 1, p.n, np, sk, tokens, p.status, s);
+    }
+    const int nt = p.n <= 8 ? 1 : 2, items = (p.n + 8 * nt - 1) / (8 * nt);
     return launch_w4_mma(0, p.dtype, g, p.w, items, items, nt, s);
 }
 

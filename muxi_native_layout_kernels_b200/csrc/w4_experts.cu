@@ -6,6 +6,8 @@
 // the 16-bit and e4m3 expert kernels.
 #include <algorithm>
 #include <cmath>
+#include <cstdio>
+#include <cstdlib>
 
 #include "moe.cuh"
 #include "w4_kernels.cuh"
@@ -79,7 +81,10 @@ int launch_w4_experts(const W4ExpertsParams& p, cudaStream_t s) {
     void* const act = ws + l.act;
     float* const scratch = reinterpret_cast<float*>(ws + l.scratch);
 
-    const int nt = slots <= 4LL * p.E ? 1 : 2, block = 8 * nt;
+    int np = 0, sk1 = 1, sk2 = 1;
+    if (slots > 8LL * p.E) np = slots > 48LL * p.E ? 128 : (slots > 24LL * p.E ? 64 : 32);
+    if (const char* v = getenv("W4_X")) sscanf(v, "%d,%d,%d", &np, &sk1, &sk2);
+    const int nt = slots <= 4LL * p.E ? 1 : 2, block = np > 0 ? np : 8 * nt;
     const int items = (int)max_items(slots, p.E, block);
     // experts that get a slot when all are as likely, and the further items of full ones: what the grid is planned for
     const int likely = std::min(items, std::max(1, (int)(p.E * (1.0 - std::exp(-(double)slots / p.E)) + (double)slots / block * 0.5)));
@@ -98,6 +103,21 @@ int launch_w4_experts(const W4ExpertsParams& p, cudaStream_t s) {
     g.k = p.H;
     g.out_tiles = p.I / 16;
     g.mat_tiles = 2 * p.I / 16;
+    MoeParams m{};
+    m.scratch = scratch; m.topk_ids = p.topk_ids; m.experts_map = p.experts_map; m.experts_map_len = p.experts_map_len;
+    m.E = p.E; m.T = p.T; m.topk = p.topk; m.H = p.H; m.y = p.y; m.y_fp32 = p.y_fp32;
+    if (np > 0) {
+        // the token rows of a work item have to be contiguous for the tile copy; the gathered rows borrow the scratch
+        if (int st = launch_moe_gather_positions(p.x, sorted, worklist, p.topk, p.H, scratch, items, s)) return st;
+        g.X = scratch;
+        if (int st = launch_w4_umma(1, p.dtype, g, p.w1, p.E, (int)slots, np, sk1, items, p.status, s)) return st;
+        g.X = act;
+        g.C = scratch;
+        g.k = p.I;
+        g.out_tiles = g.mat_tiles = p.H / 16;
+        if (int st = launch_w4_umma(2, p.dtype, g, p.w2, p.E, (int)slots, np, sk2, items, p.status, s)) return st;
+        return launch_moe_combine(m, p.dtype, s);
+    }
     if (int st = launch_w4_mma(1, p.dtype, g, p.w1, items, likely, nt, s)) return st;
     g.X = act;
     g.C = scratch;
@@ -105,9 +125,6 @@ int launch_w4_experts(const W4ExpertsParams& p, cudaStream_t s) {
     g.out_tiles = g.mat_tiles = p.H / 16;
     if (int st = launch_w4_mma(2, p.dtype, g, p.w2, items, likely, nt, s)) return st;
 
-    MoeParams m{};
-    m.scratch = scratch; m.topk_ids = p.topk_ids; m.experts_map = p.experts_map; m.experts_map_len = p.experts_map_len;
-    m.E = p.E; m.T = p.T; m.topk = p.topk; m.H = p.H; m.y = p.y; m.y_fp32 = p.y_fp32;
     return launch_moe_combine(m, p.dtype, s);
 }
 
