@@ -65,12 +65,16 @@ def _loss(x, ids, score_fun, coef, mask, cu, want_grad: bool):
     loss = x.new_empty((), dtype=torch.float32)
     counts = x.new_empty((E,), dtype=torch.int32)
     grad = torch.empty_like(x) if want_grad else None
-    head = (4 * B * E + 255) // 256 * 256          # d loss / d p [B, E] comes first: the backward pass reads it again
     nbytes = lib.mlk_router_balance_workspace_bytes(T, E, B)
-    ws = x.new_empty((head + nbytes,), dtype=torch.uint8)
-    at = ws.data_ptr()
+    # d loss / d p [B, E] comes first (the backward pass reads it again); a small batch with its gradient needs neither
+    head = 0 if want_grad and nbytes == 0 else (4 * B * E + 255) // 256 * 256
+    ws, at = None, None
+    if head:
+        ws = x.new_empty((head + nbytes,), dtype=torch.uint8)
+        at = ws.data_ptr()
     _launch(x.get_device(), lib.mlk_router_balance_loss, x.data_ptr(), ids.data_ptr(), _ptr(mask), _ptr(cu), T, E, ids.shape[1], B,
-            score_fun, coef, _CODES[x.dtype], loss.data_ptr(), counts.data_ptr(), at, _ptr(grad), at + head, nbytes)
+            score_fun, coef, _CODES[x.dtype], loss.data_ptr(), counts.data_ptr(), at, _ptr(grad), at + head if nbytes else None,
+            nbytes)
     return loss, counts, ws, grad
 
 
@@ -84,8 +88,9 @@ class _BalanceLoss(torch.autograd.Function):
         return loss, counts
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss, _):
+        if torch.is_grad_enabled():
+            raise RuntimeError("router_balance_loss can be differentiated once")
         x, dprob, mask, cu = ctx.saved_tensors
         grad = torch.empty_like(x)
         _launch(x.get_device(), lib.mlk_router_balance_grad, x.data_ptr(), _ptr(mask), _ptr(cu), x.shape[0], x.shape[1],

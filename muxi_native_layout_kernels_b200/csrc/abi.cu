@@ -581,10 +581,7 @@ int mlk_router_balance_loss(const void* logits, const int32_t* topk_ids, const v
                             int64_t workspace_bytes, mlk_stream_t s) {
     BalanceParams b{logits, topk_ids, reinterpret_cast<const uint8_t*>(token_mask), cu_seqlens, tokens, num_experts, topK,
                     sequences, score_fun, dtype, coef, loss, counts, dprob, nullptr, grad};
-    return guarded([&] {
-        if (int st = launch_balance_loss(b, workspace, workspace_bytes, (cudaStream_t)s)) return st;
-        return grad ? launch_balance_grad(b, (cudaStream_t)s) : (int)kOk;
-    });
+    return guarded([&] { return launch_balance_loss(b, workspace, workspace_bytes, (cudaStream_t)s); });
 }
 
 int mlk_router_balance_grad(const void* logits, const void* token_mask, const int32_t* cu_seqlens, int tokens, int num_experts,
