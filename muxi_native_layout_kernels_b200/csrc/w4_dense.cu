@@ -1,7 +1,5 @@
 // Products of one 4-bit matrix with n tokens: argument checks and the choice of the kernel.
 #include <algorithm>
-#include <cstdio>
-#include <cstdlib>
 
 #include "w4_kernels.cuh"
 
@@ -29,15 +27,21 @@ int launch_w4_dense(const W4DenseParams& p, cudaStream_t s) {
     g.X = p.X;
     g.C = p.C;
     g.n = p.n;
-    int np = p.n <= 32 ? 32 : (p.n <= 64 ? 64 : (p.n <= 128 ? 128 : 256)), sk = 0, lim = 16;
-    if (const char* v = getenv("W4_U")) sscanf(v, "%d,%d,%d", &lim, &np, &sk);
-    if (p.n > lim) {
-        const int tokens = (p.n + np - 1) / np, tiles = (g.out_tiles + 7) / 8, stages = (p.k + 127) / 128;
-        if (sk == 0) { sk = 1; while (sk < 8 && np <= 128 && tiles * tokens * sk < sm_count() && stages / sk >= 4) ++sk; }
-        return launch_w4_umma(0, p.dtype, g, p.w, 1, p.n, np, sk, tokens, p.status, s);
+    // Up to 16 tokens the streaming kernel, which also keeps the weights exact, above it tcgen05.  Measured on both sides:
+    // 28672 x 8192 at 8 tokens 30 us against 36 (the tcgen05 kernel's decode and hand-offs cost the same for any token
+    // count), 4096 x 14336 at 16 tokens 17.5 against 15.5, 14336 x 4096 at 61 tokens 65 against 16.8.
+    if (p.n <= 16) return launch_w4_mma(0, p.dtype, g, p.w, 1, 1, p.n <= 8 ? 1 : 2, s);
+    const W4UmmaPlan q = w4_umma_plan(g.out_tiles, p.n, p.k);
+    const int tokens = (p.n + q.np - 1) / q.np;
+    // a launch holds at most 65535 token tiles
+    for (int t0 = 0; t0 < tokens; t0 += 65535) {
+        const long long n0 = (long long)t0 * q.np;
+        g.X = reinterpret_cast<const uint8_t*>(p.X) + n0 * p.k * 2;
+        g.C = reinterpret_cast<uint8_t*>(p.C) + n0 * p.m * 2;
+        g.n = (int)std::min<long long>(p.n - n0, 65535LL * q.np);
+        if (int st = launch_w4_umma(0, p.dtype, g, p.w, 1, g.n, q.np, q.sk, 1, std::min(tokens - t0, 65535), p.status, s)) return st;
     }
-    const int nt = p.n <= 8 ? 1 : 2, items = (p.n + 8 * nt - 1) / (8 * nt);
-    return launch_w4_mma(0, p.dtype, g, p.w, items, items, nt, s);
+    return kOk;
 }
 
 }  // namespace mlk

@@ -1,14 +1,13 @@
 // The experts of a mixture layer with 4-bit weights: y[t] = sum_j p[t, j] W2_e (silu(Wg_e x_t) * (Wu_e x_t)), e = ids[t, j].
 //
-// Sequence: alignment (routed slots grouped by expert, one work item per expert and up to 8 or 16 slots) -> gate/up
-// product with SiLU on the fp32 sums -> down product, weighted, into one fp32 row per slot -> sum of a token's rows in
-// slot order with one rounding.  The activation between the two products is rounded to the 16-bit activation type, as in
+// Sequence: alignment (routed slots grouped by expert, one work item per expert and up to 8, 32, 64 or 128 slots) -> with
+// more than a few slots per expert the token rows in slot order -> gate/up product with SiLU on the fp32 sums -> down
+// product, weighted, into one fp32 row per slot -> sum of a token's rows in slot order with one rounding.  The activation between the two products is rounded to the 16-bit activation type, as in
 // the 16-bit and e4m3 expert kernels.
 #include <algorithm>
 #include <cmath>
-#include <cstdio>
-#include <cstdlib>
 
+#include "common.cuh"
 #include "moe.cuh"
 #include "w4_kernels.cuh"
 
@@ -51,6 +50,33 @@ int check_weights(const W4Weights& w, long long k, const char* name) {
     return kOk;
 }
 
+// Token row of every routed slot in position order, one warp per row (the slots behind the last routed one hold no row).
+__global__ void __launch_bounds__(256) w4_gather_kernel(const uint4* __restrict__ x, const int32_t* __restrict__ sorted, const int4* __restrict__ worklist,
+                                                        int topk, int h8, uint4* __restrict__ xg) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int pos = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (pos >= worklist[0].y) return;                    // routed slots on this rank
+    const uint4* const src = x + (size_t)(sorted[pos] / topk) * h8;
+    uint4* const dst = xg + (size_t)pos * h8;
+#pragma unroll 4
+    for (int i = lane; i < h8; i += 32) dst[i] = src[i];
+}
+
+int launch_gather(const void* x, const int32_t* sorted, const int4* worklist, int topk, int H, void* xg, long long slots, cudaStream_t s) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((slots + 7) / 8));
+    cfg.blockDim = dim3(256);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    cfg.attrs = attr;
+    cfg.numAttrs = launch_attrs(attr, 1);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, w4_gather_kernel, reinterpret_cast<const uint4*>(x), sorted, worklist, topk, H / 8,
+                                             reinterpret_cast<uint4*>(xg));
+    if (e != cudaSuccess) return fail(kCudaError, "fused_experts_compute_w4: gather launch: %s", cudaGetErrorString(e));
+    return kOk;
+}
+
 }  // namespace
 
 long long w4_experts_workspace_bytes(int T, int E, int topk, int H, int I) {
@@ -81,10 +107,12 @@ int launch_w4_experts(const W4ExpertsParams& p, cudaStream_t s) {
     void* const act = ws + l.act;
     float* const scratch = reinterpret_cast<float*>(ws + l.scratch);
 
-    int np = 0, sk1 = 1, sk2 = 1;
-    if (slots > 8LL * p.E) np = slots > 48LL * p.E ? 128 : (slots > 24LL * p.E ? 64 : 32);
-    if (const char* v = getenv("W4_X")) sscanf(v, "%d,%d,%d", &np, &sk1, &sk2);
-    const int nt = slots <= 4LL * p.E ? 1 : 2, block = np > 0 ? np : 8 * nt;
+    // Slots of a work item, by the slots an expert gets: the streaming kernel up to 4, above it tcgen05 with 32, 64 or 128.
+    // Measured (us): 2 slots 63 against 81, 4 slots 82 / 174 against 98 / 176, 8 slots 130 / 230 against 109 / 186 (128 experts of
+    // 2048 x 768 / 8 of 4096 x 14336); 32 against 64 slots a tile: 127 / 190 against 142 / 215 at 16 slots, 173 / 273
+    // against 170 / 231 at 32; 128 slots a tile: 497 against 542 at 128.
+    const int np = slots <= 4LL * p.E ? 0 : (slots <= 24LL * p.E ? 32 : (slots <= 80LL * p.E ? 64 : 128));
+    const int block = np > 0 ? np : 8;
     const int items = (int)max_items(slots, p.E, block);
     // experts that get a slot when all are as likely, and the further items of full ones: what the grid is planned for
     const int likely = std::min(items, std::max(1, (int)(p.E * (1.0 - std::exp(-(double)slots / p.E)) + (double)slots / block * 0.5)));
@@ -107,23 +135,27 @@ int launch_w4_experts(const W4ExpertsParams& p, cudaStream_t s) {
     m.scratch = scratch; m.topk_ids = p.topk_ids; m.experts_map = p.experts_map; m.experts_map_len = p.experts_map_len;
     m.E = p.E; m.T = p.T; m.topk = p.topk; m.H = p.H; m.y = p.y; m.y_fp32 = p.y_fp32;
     if (np > 0) {
+        // consecutive row tiles of a CTA of the second product: up to four where k is short and two rounds of two CTAs per SM
+        // are left (128 experts of 2048 x 768, us with 1 / 2 / 4 / 8: 113 / 107 / 106 / 106 at 128 tokens, 152 / 144 / 141 / 141
+        // at 512; with k = 14336 it only costs, 193 / 220 / 303; nor does it pay for the first product)
+        const int run = p.I > 2048 ? 1 : std::max(1, std::min(4, (int)((p.H + 127) / 128 * (long long)likely / (4LL * sm_count()))));
         // the token rows of a work item have to be contiguous for the tile copy; the gathered rows borrow the scratch
-        if (int st = launch_moe_gather_positions(p.x, sorted, worklist, p.topk, p.H, scratch, items, s)) return st;
+        if (int st = launch_gather(p.x, sorted, worklist, p.topk, p.H, scratch, slots, s)) return st;
         g.X = scratch;
-        if (int st = launch_w4_umma(1, p.dtype, g, p.w1, p.E, (int)slots, np, sk1, items, p.status, s)) return st;
+        if (int st = launch_w4_umma(1, p.dtype, g, p.w1, p.E, (int)slots, np, 1, 1, items, p.status, s)) return st;
         g.X = act;
         g.C = scratch;
         g.k = p.I;
         g.out_tiles = g.mat_tiles = p.H / 16;
-        if (int st = launch_w4_umma(2, p.dtype, g, p.w2, p.E, (int)slots, np, sk2, items, p.status, s)) return st;
+        if (int st = launch_w4_umma(2, p.dtype, g, p.w2, p.E, (int)slots, np, 1, run, items, p.status, s)) return st;
         return launch_moe_combine(m, p.dtype, s);
     }
-    if (int st = launch_w4_mma(1, p.dtype, g, p.w1, items, likely, nt, s)) return st;
+    if (int st = launch_w4_mma(1, p.dtype, g, p.w1, items, likely, 1, s)) return st;
     g.X = act;
     g.C = scratch;
     g.k = p.I;
     g.out_tiles = g.mat_tiles = p.H / 16;
-    if (int st = launch_w4_mma(2, p.dtype, g, p.w2, items, likely, nt, s)) return st;
+    if (int st = launch_w4_mma(2, p.dtype, g, p.w2, items, likely, 1, s)) return st;
 
     return launch_moe_combine(m, p.dtype, s);
 }

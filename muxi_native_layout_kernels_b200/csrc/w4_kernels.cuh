@@ -33,10 +33,15 @@ __device__ __forceinline__ void store16(void* base, size_t i, float v) {
 
 // items: work items (exact for the dense products, an upper bound for the experts, whose number the device knows);
 // likely_items: what the grid is sized for.
-// tcgen05 form: np = tokens per tile (32, 64, 128; 256 in mode 0), sk = CTAs of a cluster along k, matrices = experts (1 in
-// mode 0), x_rows = rows of X.
+// tcgen05 form: np = tokens per tile (32, 64, 128; 256 in mode 0), sk = CTAs of a cluster along k, run = consecutive
+// row tiles of a CTA, matrices = experts (1 in mode 0), x_rows = rows of X.
 int launch_w4_umma(int mode, int wt, const W4KernelParams& p, const W4Weights& w, long long matrices, int x_rows, int np, int sk,
-                   int items, int* status, cudaStream_t s);
+                   int run, int items, int* status, cudaStream_t s);
+struct W4UmmaPlan {
+    int np, sk;
+    double us;                  // estimated time
+};
+W4UmmaPlan w4_umma_plan(int rows16, int n, int k);
 int launch_w4_mma(int mode, int wt, W4KernelParams p, const W4Weights& w, int items, int likely_items, int nt, cudaStream_t s);
 
 }  // namespace mlk

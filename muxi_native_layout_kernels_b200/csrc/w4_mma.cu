@@ -337,11 +337,11 @@ const void* pick(int group, bool zp) {
     return zp ? reinterpret_cast<const void*>(w4_mma_kernel<WT, NT, kRT, kDI, 32, true, MODE>)
               : reinterpret_cast<const void*>(w4_mma_kernel<WT, NT, kRT, kDI, 32, false, MODE>);
 }
-template <int NT>
-const void* pick(int mode, int wt, int group, bool zp) {
-    if (wt == kFP16)
-        return mode == 0 ? pick<kFP16, NT, 0>(group, zp) : (mode == 1 ? pick<kFP16, NT, 1>(group, zp) : pick<kFP16, NT, 2>(group, zp));
-    return mode == 0 ? pick<kBF16, NT, 0>(group, zp) : (mode == 1 ? pick<kBF16, NT, 1>(group, zp) : pick<kBF16, NT, 2>(group, zp));
+template <int WT>
+const void* pick(int mode, int nt, int group, bool zp) {     // more than 8 slots per item of an expert go to tcgen05
+    if (mode == 0) return nt == 1 ? pick<WT, 1, 0>(group, zp) : pick<WT, 2, 0>(group, zp);
+    if (nt != 1) return nullptr;
+    return mode == 1 ? pick<WT, 1, 1>(group, zp) : pick<WT, 1, 2>(group, zp);
 }
 
 // Clusters of sk CTAs that the device holds at once.  A cluster sits inside one group of SMs, so for sk > 2 this is less
@@ -428,7 +428,8 @@ int launch_w4_mma(int mode, int wt, W4KernelParams p, const W4Weights& w, int it
     p.s = reinterpret_cast<const uint32_t*>(w.s);
     p.z = reinterpret_cast<const uint16_t*>(w.z);
     if (items > 65535) return fail(kUnsupported, "w4: %d work items exceed one launch", items);
-    const void* kern = nt == 1 ? pick<1>(mode, wt, w.group, zp) : pick<2>(mode, wt, w.group, zp);
+    const void* kern = wt == kFP16 ? pick<kFP16>(mode, nt, w.group, zp) : pick<kBF16>(mode, nt, w.group, zp);
+    if (kern == nullptr) return fail(kInvalidArg, "w4: %d tokens per item are not built", 8 * nt);
     const Plan q = cached_plan(kern, mode, nt, w.group, zp, p.out_tiles, (p.kc + 1) / 2, likely_items);
     if (q.smem == 0) return fail(kCudaError, "w4: the streaming kernel cannot be launched on this device");
     p.seg_units = q.seg;

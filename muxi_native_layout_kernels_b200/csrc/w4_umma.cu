@@ -15,6 +15,7 @@
 // between the roles, at NP = 256 the tensor pipe.  Small grids split k over a cluster; partial tiles are added through
 // distributed shared memory in a fixed order.
 #include <algorithm>
+#include <cmath>
 
 #include "umma_common.cuh"
 #include "w4_kernels.cuh"
@@ -45,6 +46,7 @@ constexpr int token_stages(int np) { return np >= 256 ? 2 : (np >= 128 ? 2 : 3);
 struct UmmaParams {
     W4KernelParams k;
     int stages;                 // stages of 128 k
+    int run;                    // consecutive row tiles of a CTA (1 where a cluster splits k)
     int sbytes;                 // bytes of a raw stage and weight tile: packed, scales, zero points
     int* status;
 };
@@ -94,13 +96,18 @@ __global__ void __launch_bounds__(kThreads, tmem_columns(MODE == 1 ? 2 : 1, NP) 
     constexpr uint32_t kTmemCols = tmem_columns(NA, NP);
     constexpr int kTile = kRaw + 256 * NG + (ZP ? 128 * NG : 0);      // raw stage of one weight tile
     constexpr int kB = NP * 256;                                     // token tile of a stage: two 64-k halves
-    __shared__ __align__(8) uint64_t bars[2 * RS + 2 * S2 + 2 * SB + 1];
+    __shared__ __align__(8) uint64_t bars[2 * RS + 2 * S2 + 2 * SB + 2];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_flag;
+    // MODE 2: slot and routing weight of every token of the item (fetched where they are used, each column of the read-out
+    // waited for two dependent loads behind the stores of the one before: 10 us for 16 columns)
+    __shared__ int slot_of[MODE == 2 ? NP : 1];
+    __shared__ float weight_of[MODE == 2 ? NP : 1];
 
     const W4KernelParams& p = u.k;
     const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
-    const int tile = blockIdx.x, rank = blockIdx.y, SK = gridDim.y;
+    const int row_tiles = (p.out_tiles + 7) / 8, tile = blockIdx.x * u.run, rank = blockIdx.y, SK = gridDim.y;
+    const int run = min(u.run, row_tiles - tile);
 
     const bool early = MODE == 0 && static_weights;
     if (!early) {
@@ -117,7 +124,15 @@ __global__ void __launch_bounds__(kThreads, tmem_columns(MODE == 1 ? 2 : 1, NP) 
         if ((int)blockIdx.z >= items) return;    // uniform over the cluster
         mat = item.x; pos0 = item.y; ntok = item.z; row0 = item.w;
     }
+    if constexpr (MODE == 2) {
+        for (int c = tid; c < ntok; c += kThreads) {
+            const int slot = p.sorted[pos0 + c];
+            slot_of[c] = slot;
+            weight_of[c] = load_scalar16<WT>(p.topk_weights, slot);
+        }
+    }
     const int st0 = (int)((long long)u.stages * rank / SK), n = (int)((long long)u.stages * (rank + 1) / SK) - st0;
+    const int total = n * run;                   // stages of all row tiles, one after the other
 
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* const base_ptr = smem_raw + (base - smem_u32(smem_raw));
@@ -129,7 +144,7 @@ __global__ void __launch_bounds__(kThreads, tmem_columns(MODE == 1 ? 2 : 1, NP) 
     auto cv_empty = [&](int s) { return bar0 + 8u * (2 * RS + S2 + s); };
     auto x_full = [&](int s) { return bar0 + 8u * (2 * RS + 2 * S2 + s); };
     auto x_empty = [&](int s) { return bar0 + 8u * (2 * RS + 2 * S2 + SB + s); };
-    const uint32_t acc_full = bar0 + 8u * (2 * RS + 2 * S2 + 2 * SB);
+    const uint32_t acc_full = bar0 + 8u * (2 * RS + 2 * S2 + 2 * SB), acc_empty = acc_full + 8u;
 
     if (tid == 0) {
         for (int s = 0; s < RS; ++s) {
@@ -145,6 +160,7 @@ __global__ void __launch_bounds__(kThreads, tmem_columns(MODE == 1 ? 2 : 1, NP) 
             mbar_init(x_empty(s), 1);            // tcgen05.commit
         }
         mbar_init(acc_full, 1);
+        mbar_init(acc_empty, kConv);             // one arrival per warp that has read its part
         abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -159,18 +175,54 @@ __global__ void __launch_bounds__(kThreads, tmem_columns(MODE == 1 ? 2 : 1, NP) 
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, tmem_slot, 0);
 
+    // ---- read-out of one row tile where this CTA has the whole sums: set 0 the lower half of the tokens, set 1 the upper,
+    // straight from tensor memory, a thread has one row, neighbouring lanes neighbouring rows ----
+    const size_t ld = (size_t)p.out_tiles * 16;
+    auto silu_mul = [](float g, float h) { return g / (1.f + __expf(-g)) * h; };
+    auto read_out = [&](int rt, int quad, int set) {
+        const int lrow = quad * 32 + lane, row = rt * kTileM + lrow;
+        const float f = (lrow & 8) ? D::kFactorHigh : D::kFactorLow;   // the decode's constant factor of this row
+        const uint32_t at = tmem + ((uint32_t)(quad * 32) << 16);
+        const bool mine = row < p.out_tiles * 16;
+        const float alpha = MODE == 0 ? f * p.alpha : f;
+        const float bias = MODE == 0 && mine && p.bias ? load_scalar16<WT>(p.bias, row) : 0.f;
+        uint16_t* out = reinterpret_cast<uint16_t*>(p.C) + (size_t)(row0 + set * (NP / 2)) * ld + row;
+#pragma unroll 1
+        for (int c0 = set * (NP / 2); c0 < (set + 1) * (NP / 2) && c0 < ntok; c0 += 16) {
+            uint32_t a[16], b[16];
+            tmem_ld16(at + c0, a);
+            if constexpr (NA == 2) tmem_ld16(at + NP + c0, b);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            const int left = mine ? ntok - c0 : 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                if (i < left) {
+                    const float v = __uint_as_float(a[i]);
+                    if constexpr (MODE == 0) {
+                        store16<WT>(out, 0, fmaf(alpha, v, bias));
+                    } else if constexpr (MODE == 1) {
+                        store16<WT>(out, 0, silu_mul(f * v, f * __uint_as_float(b[i])));
+                    } else {
+                        reinterpret_cast<float*>(p.C)[(size_t)slot_of[c0 + i] * ld + row] = weight_of[c0 + i] * (f * v);
+                    }
+                }
+                out += ld;
+            }
+        }
+    };
+
     int raw_issued = 0, x_issued = 0;
     if (warp == 0) {
         // ---- TMA producer: raw weights and token tiles are two independent streams, polled without blocking ----
         const uint64_t wpol = l2_evict_first_policy();
         const int g16 = mat * p.mat_tiles + tile * 8;                  // first 16-row group
-        auto load_raw = [&](int i, int s) {
+        auto load_raw = [&](int i, int t, int s) {   // stage i of row tile t of the run
             if (elect_one()) {
                 mbar_expect_tx(raw_full(s), NA * kTile);
 #pragma unroll
                 for (int w = 0; w < NA; ++w) {
                     const uint32_t dst = r_base + (s * NA + w) * kTile;
-                    const int g = g16 + (w == 1 ? p.out_tiles : 0);
+                    const int g = g16 + t * 8 + (w == 1 ? p.out_tiles : 0);
                     tma_load_3d_hint(dst, &map_q, raw_full(s), 0, (st0 + i) * 2, g, wpol);
                     tma_load_3d(dst + kRaw, &map_s, raw_full(s), 0, (st0 + i) * NG, g);
                     if constexpr (ZP) tma_load_3d(dst + kRaw + 256 * NG, &map_z, raw_full(s), 0, (st0 + i) * NG, g);
@@ -179,31 +231,37 @@ __global__ void __launch_bounds__(kThreads, tmem_columns(MODE == 1 ? 2 : 1, NP) 
             __syncwarp();
         };
         int ri = 0, xi = 0, rs = 0, xs = 0;      // next stage of each stream and its ring slot
+        int rk = 0, rt = 0, xk = 0;              // the same as (stage, row tile)
         uint32_t rpar = 1, xpar = 1;             // parity that says the slot is free: the first round finds it so
         if (early) {
-            for (; ri < min(n, RS); ++ri) load_raw(ri, ri);
+            for (; ri < min(total, RS); ++ri) {
+                load_raw(rk, rt, ri);
+                if (++rk == n) { rk = 0; ++rt; }
+            }
             if (ri == RS) rpar ^= 1u;
             rs = ri % RS;
             pdl_launch_dependents();
             pdl_wait();
         }
         uint32_t idle = 0;
-        while ((xi < n || ri < n) && !__any_sync(kAll, abort_flag)) {
+        while ((xi < total || ri < total) && !__any_sync(kAll, abort_flag)) {
             bool progressed = false;
-            if (ri < n && __any_sync(kAll, mbar_test_wait(raw_empty(rs), rpar))) {
-                load_raw(ri, rs);
+            if (ri < total && __any_sync(kAll, mbar_test_wait(raw_empty(rs), rpar))) {
+                load_raw(rk, rt, rs);
                 ++ri;
+                if (++rk == n) { rk = 0; ++rt; }
                 if (++rs == RS) { rs = 0; rpar ^= 1u; }
                 progressed = true;
             }
-            if (xi < n && __any_sync(kAll, mbar_test_wait(x_empty(xs), xpar))) {
+            if (xi < total && __any_sync(kAll, mbar_test_wait(x_empty(xs), xpar))) {
                 if (elect_one()) {
                     mbar_expect_tx(x_full(xs), kB);
-                    tma_load_2d(x_base + xs * kB, &map_x, x_full(xs), (st0 + xi) * kStageK, row0);
-                    tma_load_2d(x_base + xs * kB + NP * 128, &map_x, x_full(xs), (st0 + xi) * kStageK + 64, row0);
+                    tma_load_2d(x_base + xs * kB, &map_x, x_full(xs), (st0 + xk) * kStageK, row0);
+                    tma_load_2d(x_base + xs * kB + NP * 128, &map_x, x_full(xs), (st0 + xk) * kStageK + 64, row0);
                 }
                 __syncwarp();
                 ++xi;
+                if (++xk == n) xk = 0;
                 if (++xs == SB) { xs = 0; xpar ^= 1u; }
                 progressed = true;
             }
@@ -226,9 +284,13 @@ __global__ void __launch_bounds__(kThreads, tmem_columns(MODE == 1 ? 2 : 1, NP) 
         const uint64_t d0 = smem_desc(x_base, 16, 1024, 2);
         const uint32_t a0 = tmem + NA * NP;
         int s2 = 0, sb = 0;
-        uint32_t par2 = 0, parb = 0;
-        for (int i = 0; i < n; ++i) {
-            const bool ready = mbar_wait(x_full(sb), parb) && mbar_wait(cv_full(s2), par2);
+        uint32_t par2 = 0, parb = 0, para = 1;   // para: the parity that says the accumulator is free
+        for (int f = 0, i = 0; f < total; ++f) {
+            bool ready = mbar_wait(x_full(sb), parb) && mbar_wait(cv_full(s2), par2);
+            if (i == 0) {
+                ready = ready && mbar_wait(acc_empty, para);
+                para ^= 1u;
+            }
             if (__any_sync(kAll, !ready || abort_flag)) {
                 if (!abort_flag && u.status && lane == 0) atomicExch(u.status, 2);
                 abort_flag = 1;
@@ -249,6 +311,7 @@ __global__ void __launch_bounds__(kThreads, tmem_columns(MODE == 1 ? 2 : 1, NP) 
                 if (i == n - 1) umma_commit(acc_full);
             }
             __syncwarp();
+            if (++i == n) i = 0;
             if (++s2 == S2) { s2 = 0; par2 ^= 1u; }
             if (++sb == SB) { sb = 0; parb ^= 1u; }
         }
@@ -258,8 +321,10 @@ __global__ void __launch_bounds__(kThreads, tmem_columns(MODE == 1 ? 2 : 1, NP) 
         const int quad = warp & 3, set = (warp - 2) >> 2, r = lane >> 2;
         constexpr int kStep = NA == 2 ? 1 : 2;   // stages of a set
         int s = NA == 2 ? 0 : set, s2 = s % S2;
-        uint32_t parr = 0, par2 = 1;             // par2: the parity that says the slot is free
-        for (int i = s; i < n; i += kStep) {
+        uint32_t parr = 0, par2 = 1, para = 0;   // par2: the parity that says the slot is free
+        int f = s;
+        for (int t = 0; t < run; ++t) {
+          for (; f < (t + 1) * n; f += kStep) {
             bool ok = mbar_wait(raw_full(s), parr) && !abort_flag;
             uint32_t v[32];
 #pragma unroll
@@ -310,58 +375,29 @@ __global__ void __launch_bounds__(kThreads, tmem_columns(MODE == 1 ? 2 : 1, NP) 
             if (s >= RS) { s -= RS; parr ^= 1u; }
             s2 += kStep;
             if (s2 >= S2) { s2 -= S2; par2 ^= 1u; }
+          }
+            // the row tile's accumulator is complete
+            if (__any_sync(kAll, abort_flag || !mbar_wait(acc_full, para))) {
+                if (!abort_flag && u.status && lane == 0) atomicExch(u.status, 3);
+                abort_flag = 1;
+                break;
+            }
+            para ^= 1u;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (SK > 1) break;                   // read out below, with the cluster
+            read_out(tile + t, quad, set);
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(acc_empty) : "memory");
         }
-        __syncwarp();
-        if (__any_sync(kAll, abort_flag || !mbar_wait(acc_full, 0))) {
-            if (!abort_flag && u.status && lane == 0) atomicExch(u.status, 3);
-            abort_flag = 1;
-        }
-        __syncwarp();
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     }
     __syncwarp();
 
-    // ---- epilogue: set 0 the lower half of the tokens, set 1 the upper ----
-    const size_t ld = (size_t)p.out_tiles * 16;
-    const int rows_left = p.out_tiles * 16 - tile * kTileM;            // rows of the matrix in this tile
-    auto silu_mul = [](float g, float h) { return g / (1.f + __expf(-g)) * h; };
-    constexpr int kChunk = NP < 64 ? NP : 64;                          // tokens of one pass through shared memory
-    if (SK == 1) {
-        // straight from tensor memory: a thread has one row, neighbouring lanes neighbouring rows
-        if (warp >= 2 && !abort_flag) {
-            const int quad = warp & 3, set = (warp - 2) >> 2, lrow = quad * 32 + lane, row = tile * kTileM + lrow;
-            const float f = (lrow & 8) ? D::kFactorHigh : D::kFactorLow;
-            const uint32_t at = tmem + ((uint32_t)(quad * 32) << 16);
-            const bool mine = lrow < rows_left;
-            const float alpha = MODE == 0 ? f * p.alpha : f;
-            const float bias = MODE == 0 && mine && p.bias ? load_scalar16<WT>(p.bias, row) : 0.f;
-            uint16_t* out = reinterpret_cast<uint16_t*>(p.C) + (size_t)(row0 + set * (NP / 2)) * ld + row;
-#pragma unroll 1
-            for (int c0 = set * (NP / 2); c0 < (set + 1) * (NP / 2) && c0 < ntok; c0 += 16) {
-                uint32_t a[16], b[16];
-                tmem_ld16(at + c0, a);
-                if constexpr (NA == 2) tmem_ld16(at + NP + c0, b);
-                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                const int left = mine ? ntok - c0 : 0;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    if (i < left) {
-                        const float v = __uint_as_float(a[i]);
-                        if constexpr (MODE == 0) {
-                            store16<WT>(out, 0, fmaf(alpha, v, bias));
-                        } else if constexpr (MODE == 1) {
-                            store16<WT>(out, 0, silu_mul(f * v, f * __uint_as_float(b[i])));
-                        } else {
-                            const int slot = p.sorted[pos0 + c0 + i];
-                            reinterpret_cast<float*>(p.C)[(size_t)slot * ld + row] = load_scalar16<WT>(p.topk_weights, slot) * (f * v);
-                        }
-                    }
-                    out += ld;
-                }
-            }
-        }
-    } else {
-        // partial tiles [which][token][row] of a chunk of tokens in the (idle) rings, added over the cluster in rank order
+    // ---- cluster: partial tiles over the k parts ----
+    if (SK > 1) {
+        const int rows_left = p.out_tiles * 16 - tile * kTileM;        // rows of the matrix in this tile
+        constexpr int kChunk = NP < 64 ? NP : 64;                      // tokens of one pass through shared memory
+        // [which][token][row] of a chunk of tokens in the (idle) rings, added over the cluster in rank order
         float* const red = reinterpret_cast<float*>(base_ptr);
         uint32_t remote[8];
 #pragma unroll
@@ -416,9 +452,8 @@ __global__ void __launch_bounds__(kThreads, tmem_columns(MODE == 1 ? 2 : 1, NP) 
                         make_uint2(pack2<WT>(silu_mul(v[0].x, v[NA - 1].x), silu_mul(v[0].y, v[NA - 1].y)),
                                    pack2<WT>(silu_mul(v[0].z, v[NA - 1].z), silu_mul(v[0].w, v[NA - 1].w)));
                 } else {
-                    const int slot = p.sorted[pos0 + cb + c];
-                    const float t = load_scalar16<WT>(p.topk_weights, slot);
-                    *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.C) + (size_t)slot * ld + row) =
+                    const float t = weight_of[cb + c];
+                    *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.C) + (size_t)slot_of[cb + c] * ld + row) =
                         make_float4(t * v[0].x, t * v[0].y, t * v[0].z, t * v[0].w);
                 }
             }
@@ -495,11 +530,36 @@ bool map_groups(CUtensorMap* m, const void* v, long long groups16, int groups, i
     });
 }
 
+// Estimated time (us) of a product: a CTA costs 5 us to start and to read out (1 more with a cluster), a stage of 128 k on an
+// SM the time below, whatever the number of CTAs that share it, and rounds are whole.  (Fitted to sweeps over 4096 x 4096 ..
+// 28672 x 8192 at 8 to 500 tokens; within 15 % there.)
+double stage_us(int np) { return np == 32 ? 0.33 : (np == 64 ? 0.37 : (np == 128 ? 0.51 : 0.70)); }
+double estimate(int tiles, int tokens, int stages, int np, int sk) {
+    const double ctas = (double)tiles * tokens * sk, resident = np == 256 ? 1.0 : 2.0;
+    const double slots = sm_count() * resident * (sk > 2 ? 0.9 : 1.0);     // clusters of more than two do not fill every SM
+    const double rounds = std::ceil(ctas / slots), share = std::min(resident, std::ceil(ctas / sm_count()));
+    return rounds * (5.0 + (sk > 1 ? 1.0 : 0.0) + std::ceil((double)stages / sk) * stage_us(np) * share);
+}
+
 }  // namespace
 
+W4UmmaPlan w4_umma_plan(int rows16, int n, int k) {
+    const int tiles = (rows16 + 7) / 8, stages = (k + kStageK - 1) / kStageK;
+    W4UmmaPlan best{32, 1, 1e30};
+    for (int np = 32; np <= 256; np *= 2) {
+        const int tokens = (n + np - 1) / np;
+        for (int sk = 1; sk <= (np == 256 ? 1 : 8) && sk <= stages; ++sk) {
+            const double us = estimate(tiles, tokens, stages, np, sk);
+            if (us < best.us) best = W4UmmaPlan{np, sk, us};
+        }
+        if (tokens == 1) break;                  // a wider tile would only compute more columns that nobody reads
+    }
+    return best;
+}
+
 // One product.  mode 0: X = tokens [n, k]; mode 1: X = gathered tokens [x_rows, k]; mode 2: X = activations [x_rows, k].
-// np: token tile; sk: CTAs of a cluster along k; items: token tiles (mode 0) or an upper bound of the work items.
-int launch_w4_umma(int mode, int wt, const W4KernelParams& kp, const W4Weights& w, long long matrices, int x_rows, int np, int sk,
+// np: token tile; sk: CTAs of a cluster along k; run: consecutive row tiles of a CTA; items: token tiles (mode 0) or an upper bound of the work items.
+int launch_w4_umma(int mode, int wt, const W4KernelParams& kp, const W4Weights& w, long long matrices, int x_rows, int np, int sk, int run,
                    int items, int* status, cudaStream_t s) {
     const bool zp = w.z != nullptr;
     UmmaParams u{};
@@ -507,10 +567,12 @@ int launch_w4_umma(int mode, int wt, const W4KernelParams& kp, const W4Weights& 
     u.k.kc = (kp.k + kW4BlockK - 1) / kW4BlockK;
     u.k.groups = kp.k / w.group;
     u.stages = (u.k.kc + 1) / 2;
+    u.run = std::max(1, std::min(run, (kp.out_tiles + 7) / 8));
     u.status = status;
     const void* kern = wt == kFP16 ? pick<kFP16>(mode, np, w.group, zp) : pick<kBF16>(mode, np, w.group, zp);
     if (kern == nullptr) return fail(kInvalidArg, "w4 (tcgen05): token tile %d is not built", np);
     if (sk < 1 || sk > 8 || sk > u.stages) return fail(kInvalidArg, "w4 (tcgen05): cluster size %d out of range", sk);
+    if (sk > 1 && u.run > 1) return fail(kInvalidArg, "w4 (tcgen05): a cluster takes one row tile");
     if (sk > 1 && np > 128) return fail(kInvalidArg, "w4 (tcgen05): k is not split with %d tokens per tile", np);
     if (encode_fn() == nullptr) return fail(kUnsupported, "w4 (tcgen05): cuTensorMapEncodeTiled is not available");
     if (items > 65535) return fail(kUnsupported, "w4 (tcgen05): %d work items exceed one launch", items);
@@ -533,7 +595,8 @@ int launch_w4_umma(int mode, int wt, const W4KernelParams& kp, const W4Weights& 
     if (smem == 0) return fail(kCudaError, "w4 (tcgen05): a CTA with %d tokens does not fit on this device", np);
     int static_weights = option(kOptStaticWeights);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((kp.out_tiles + 7) / 8), (unsigned)sk, (unsigned)items);
+    const int row_tiles = (kp.out_tiles + 7) / 8;
+    cfg.gridDim = dim3((unsigned)((row_tiles + u.run - 1) / u.run), (unsigned)sk, (unsigned)items);
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
