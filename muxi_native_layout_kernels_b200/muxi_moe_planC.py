@@ -8,7 +8,8 @@ Same signature and semantics as the reference's ``muxi_layout_kernels.muxi_moe_p
   * ``w1_scale``/``w2_scale`` may be ``None`` with ``soft_fp8=True`` (unit scales);
   * each token's expert outputs are summed in fp32 in a fixed order and rounded once (``deterministic=True``,
     the default); ``deterministic=False`` accumulates into ``y`` with 16-bit atomics like the reference;
-  * the launch sequence is 5 kernels (router, alignment, GEMM1+SiLU, GEMM2, combine) instead of 6.
+  * the launch sequence is 5 kernels (router, alignment, GEMM1+SiLU, GEMM2, combine) instead of 6;
+  * ``fused_moe_w4`` is the same layer on expert weights in 4 bits with group scales.
 """
 from __future__ import annotations
 
@@ -20,6 +21,7 @@ import csv
 from pathlib import Path
 
 from . import ext
+from .w4 import fused_experts_compute_w4
 
 # Launch arguments of the expert-compute kernels, tuned offline by kernel_args_scan/moe_scan.py (the reference tunes
 # its MoE tile arguments with kernel_args_scan/muxi_moe_args_scan.py and bakes them into this function's defaults).
@@ -225,6 +227,59 @@ def _experts(soft_fp8, w1, w2, hidden_states, B, e1, topk, topk_ids, topk_weight
                                   splitK=splitK, tile_m_2=tile_m_2, tile_n_2=tile_n_2, tile_k_2=tile_k_2,
                                   block_dim_x_gemm=block_dim_x_gemm, experts_map=experts_map,
                                   deterministic=deterministic, tune=tune, routing=routing)
+
+
+def fused_moe_w4(
+    hidden_states: torch.Tensor,   # [batch_size, hidden_size] bf16 / fp16
+    w1: torch.Tensor,              # [E, 2I/16, ceil(H/64), 32, 16] from layoutA_w4 (gate rows first, then up rows)
+    w2: torch.Tensor,              # [E, H/16, ceil(I/64), 32, 16]
+    gating_output: torch.Tensor,   # [batch_size, num_experts] router logits
+    topk: int,
+    renormalize: bool,
+    use_grouped_topk: bool = False,
+    num_expert_group: Optional[int] = None,
+    topk_group: Optional[int] = None,
+    w1_scale: torch.Tensor = None,   # [E, 2I/16, H/group, 8, 2] from layoutA_w4_groups, in the activations' type
+    w2_scale: torch.Tensor = None,   # [E, H/16, I/group, 8, 2]
+    w1_zeros: Optional[torch.Tensor] = None,
+    w2_zeros: Optional[torch.Tensor] = None,
+    gating_bias: Optional[torch.Tensor] = None,
+    score_func: str = "softmax",
+    experts_map: Optional[torch.Tensor] = None,
+    gate_weight: Optional[torch.Tensor] = None,
+    out_dtype: Optional[torch.dtype] = None,
+    out: Optional[torch.Tensor] = None,
+    return_routing: bool = False,
+):
+    """The layer of ``fused_moe`` with expert weights in 4 bits and group scales: router (with the renormalisation of the
+    top-k weights), then ``fused_experts_compute_w4``.  Same routing arguments; no host synchronisation, capturable in a
+    CUDA graph.  ``return_routing=True`` gives ``(y, topk_ids, topk_weights)``, for ``expert_counts`` (load statistics of a
+    server) or ``router_balance_loss``.  The reference has no counterpart."""
+    assert gate_weight is not None or hidden_states.shape[0] == gating_output.shape[0], "Number of tokens mismatch"
+    if w1_scale is None or w2_scale is None:
+        raise ValueError("4-bit weights need their group scales")
+    if not use_grouped_topk and num_expert_group not in (None, 1):
+        raise ValueError("When use_grouped_topk is False, num_expert_group must be 1.")
+    if score_func not in ("softmax", "sigmoid"):
+        raise ValueError("Unsupported scoring function")
+    B, H = hidden_states.shape
+    topk_ids = hidden_states.new_empty((B, topk), dtype=torch.int32)
+    topk_weights = hidden_states.new_empty((B, topk))
+    score_fun, groups, kept = int(score_func == "sigmoid"), num_expert_group or 1, topk_group or 1
+    if B > 0:
+        with _Range("planC.router"):
+            if gate_weight is not None:
+                ext.fused_router_gemm_gate(hidden_states, gate_weight, score_fun, groups, kept, topk_ids, topk_weights, topk,
+                                           gating_bias, renormalize=bool(renormalize))
+            else:
+                ext.fused_routing_gate(gating_output, score_fun, B, H, groups, kept, topk_ids, topk_weights, topk, gating_bias,
+                                       renormalize=bool(renormalize))
+    if experts_map is not None and experts_map.dtype != torch.int:
+        experts_map = experts_map.to(torch.int)
+    with _Range("planC.experts"):
+        y = fused_experts_compute_w4(w1, w1_scale, w2, w2_scale, hidden_states, topk_ids, topk_weights, w1_zeros, w2_zeros,
+                                     experts_map, out, out_dtype)
+    return (y, topk_ids, topk_weights) if return_routing else y
 
 
 class GraphedFusedMoE:

@@ -2,7 +2,8 @@
 
 ``fused_moe`` is the dense, per-expert torch formulation of the MoE layer that the reference's tests compare the
 fused kernels with (utils.py:131-244); ``scale_tensor`` / ``scale_whole_tensor`` expand 128x128 block scales
-(utils.py:7-25).  None of this is used by the CUDA path of this package; it exists so that code written against
+(utils.py:7-25).  ``quantize_w4`` / ``dequantize_w4`` make and undo 4-bit weights with group scales (no counterpart in the
+reference).  None of this is used by the CUDA path of this package; it exists so that code written against
 the reference package (its tests, its benchmarks) keeps importing and running.
 """
 from __future__ import annotations
@@ -27,6 +28,36 @@ def scale_whole_tensor(weight: torch.Tensor, scale: torch.Tensor) -> torch.Tenso
     """Per-expert ``scale_tensor`` of ``weight[E,m,k]`` after converting it to bf16."""
     w = weight.to(torch.bfloat16)
     return torch.stack([scale_tensor(w[e], scale[e]) for e in range(w.shape[0])])
+
+
+def quantize_w4(weight: torch.Tensor, group_size: int = 128, zero_points: bool = False):
+    """``weight[..., m, k]`` to 4 bits with group scales, round to nearest: ``(qweight, scales, zeros)`` with ``qweight``
+    uint8 ``[..., m, k/2]`` (low nibble = even k), ``scales [..., m, k/group_size]`` in weight's dtype and ``zeros`` uint8 or
+    None.  Without zero points the values are symmetric around 8 (scale = largest magnitude / 7); with them the range of the
+    group, widened to hold 0, is mapped to 0..15.  A group of zeros gets the scale 1."""
+    *lead, m, k = weight.shape
+    if k % group_size != 0 or group_size not in (32, 64, 128):
+        raise ValueError("groups of 32, 64 or 128 that divide k")
+    w = weight.to(torch.float32).reshape(*lead, m, k // group_size, group_size)
+    if zero_points:
+        lo, hi = w.amin(-1).clamp_max(0), w.amax(-1).clamp_min(0)
+        s = (hi - lo) / 15
+    else:
+        s = w.abs().amax(-1) / 7
+    s = s.to(weight.dtype)
+    s = torch.where(s == 0, torch.ones_like(s), s)
+    f = s.to(torch.float32)
+    z = torch.round(-lo / f).clamp(0, 15) if zero_points else torch.full_like(f, 8.0)
+    q = torch.round(w / f.unsqueeze(-1) + z.unsqueeze(-1)).clamp(0, 15).to(torch.uint8).reshape(*lead, m, k)
+    return q[..., 0::2] | (q[..., 1::2] << 4), s, z.to(torch.uint8) if zero_points else None
+
+
+def dequantize_w4(qweight: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``[..., m, k]`` in fp32 from what ``quantize_w4`` returns: ``(q - z) * s``, z = 8 without zero points."""
+    q = torch.stack((qweight & 15, qweight >> 4), -1).flatten(-2).to(torch.float32)
+    group = q.shape[-1] // scales.shape[-1]
+    z = 8.0 if zeros is None else zeros.to(torch.float32).repeat_interleave(group, -1)
+    return (q - z) * scales.to(torch.float32).repeat_interleave(group, -1)
 
 
 def _route(gating_output, topk, num_expert_group, topk_group, renormalize, bias, score_func, dtype):
