@@ -85,12 +85,15 @@ class _BalanceLoss(torch.autograd.Function):
         ctx.save_for_backward(x, dprob, mask, cu)
         ctx.score_fun = score_fun
         ctx.mark_non_differentiable(counts)
+        ctx.set_materialize_grads(False)          # else every backward pass fills zeros for the counts
         return loss, counts
 
     @staticmethod
     def backward(ctx, grad_loss, _):
         if torch.is_grad_enabled():
             raise RuntimeError("router_balance_loss can be differentiated once")
+        if grad_loss is None:
+            return None, None, None, None, None, None
         x, dprob, mask, cu = ctx.saved_tensors
         grad = torch.empty_like(x)
         _launch(x.get_device(), lib.mlk_router_balance_grad, x.data_ptr(), _ptr(mask), _ptr(cu), x.shape[0], x.shape[1],

@@ -12,27 +12,31 @@
 //             grow along the tokens: no buffer has to be cleared and no float is added by an atomic
 //   finish    one cluster of eight CTAs, a slice of the experts each: records -> counts, u, loss, in a fixed order
 //   grad      the runs again: p recomputed, u in, gradient out
-// and for small batches one CTA that keeps p in shared memory and does all three steps in one launch.
-// What bounds it: at large T the latency of a row (load, two reductions over its lanes) and the logits' traffic (two
-// reads, one write), below some thousand tokens the launches.  A row's 16-byte loads are spread over as few lanes as
-// cover it (8 experts in bf16: one lane per token), so that a warp holds up to 32 tokens, and a warp takes kRows such
-// groups of rows at a time so that their loads and reductions overlap.
+// and for small batches one launch, a CTA or a cluster of eight that keeps p in shared memory and does all three steps.
+// What bounds it: latency, of a row (load, two reductions over its lanes) and of the launches; the logits' traffic (two
+// reads, one write) is a few microseconds at the largest sizes.  A row's 16-byte loads are spread over as few lanes as
+// cover it (8 experts in bf16: one lane per token), so that a warp holds up to 32 tokens.  Rows are overlapped by warps, not
+// inside a warp: with four row groups unrolled the code of these kernels, run once per launch, waited for its own
+// instructions (192 x 8 in one CTA: 8.6 us against 4.0).
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "common.cuh"
 #include "moe_balance.cuh"
 #include "status.h"
+#include "umma_common.cuh"
 
 namespace mlk {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;
 constexpr int kFinishThreads = 1024;
 constexpr int kSmallThreads = 512;
-constexpr int kSmallElems = 8192;    // p of a small batch in shared memory (32 KB; no more than 48 KB with all else)
+constexpr int kSmallElems = 16384;   // scores of a CTA's tokens in a small batch, in shared memory
 constexpr int kSmallSums = 1024;     // (sequence, expert) pairs of a small batch
+constexpr int kSmallCluster = 8;
 constexpr int kFinishCtas = 8;
 constexpr int kF32 = 3;          // dtype code of fp32 logits in this file
 
@@ -44,6 +48,7 @@ struct Params {
     int T, E, topk, B, score_fun;
     int R;                       // tokens per run
     int lpr;                     // lanes per row
+    int cw, parts, per;          // finish: experts per CTA, threads per expert, threads per expert and sequence
     float coef;
     float* P;                    // records
     int32_t* C;
@@ -155,11 +160,8 @@ __device__ __forceinline__ void scores(const Params& p, float (&x)[N], float (&o
     for (int i = 0; i < N; ++i) x[i] *= inv;
 }
 
-// Row groups that a warp works on at once.
-constexpr int rows_at_once(int n) { return n <= 8 ? 4 : (n <= 16 ? 2 : 1); }
-
 template <int DT, int V, int J>
-__global__ void __launch_bounds__(kThreads, V * J <= 8 ? 4 : 1) balance_partial_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads) balance_partial_kernel(const Params p) {
     constexpr int N = V * J;
     extern __shared__ __align__(16) uint8_t smem[];
     float* const sP = reinterpret_cast<float*>(smem);                       // [warps][E]
@@ -181,41 +183,28 @@ __global__ void __launch_bounds__(kThreads, V * J <= 8 ? 4 : 1) balance_partial_
 #pragma unroll
         for (int i = 0; i < N; ++i) acc[i] = 0.f;
         int n = 0;
-        constexpr int RB = rows_at_once(N);
-        const int step = (kThreads / 32) * rows_per_warp;                   // rows of all warps' groups
-        for (int r0 = a + warp * rows_per_warp + group; r0 - group < z; r0 += RB * step) {
-            // logits, masks and picks of all rows on their way before the first is used; what is not counted becomes -inf
-            float x[RB][N], unused[1];
-            bool live[RB];
-            int pick[RB];
-#pragma unroll
-            for (int q = 0; q < RB; ++q) {
-                const int row = r0 + q * step;
-                live[q] = row < z;
-                load_row<DT, V, J>(p, row, sub, live[q], x[q]);
-                pick[q] = live[q] && sub < p.topk ? p.ids[(long long)row * p.topk + sub] : -1;
-                if (p.mask != nullptr && live[q]) live[q] = p.mask[row] != 0;
-            }
-#pragma unroll
-            for (int q = 0; q < RB; ++q) {
-                if (live[q]) {
-                    if (pick[q] >= 0 && pick[q] < p.E) atomicAdd(&sC[pick[q]], 1);
-                    for (int j = sub + p.lpr; j < p.topk; j += p.lpr) {
-                        const int e = p.ids[(long long)(r0 + q * step) * p.topk + j];
-                        if (e >= 0 && e < p.E) atomicAdd(&sC[e], 1);
-                    }
-                    n += sub == 0;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < N; ++i) x[q][i] = -INFINITY;
+        for (int r0 = a + warp * rows_per_warp; r0 < z; r0 += (kThreads / 32) * rows_per_warp) {
+            // logits, mask and picks on their way before the first is used; what is not counted becomes -inf
+            const int row = r0 + group;
+            bool live = row < z;
+            float x[N], unused[1];
+            load_row<DT, V, J>(p, row, sub, live, x);
+            const int pick = live && sub < p.topk ? p.ids[(long long)row * p.topk + sub] : -1;
+            if (p.mask != nullptr && live) live = p.mask[row] != 0;
+            if (live) {
+                if (pick >= 0 && pick < p.E) atomicAdd(&sC[pick], 1);
+                for (int j = sub + p.lpr; j < p.topk; j += p.lpr) {
+                    const int e = p.ids[(long long)row * p.topk + j];
+                    if (e >= 0 && e < p.E) atomicAdd(&sC[e], 1);
                 }
-            }
+                n += sub == 0;
+            } else {
 #pragma unroll
-            for (int q = 0; q < RB; ++q) {
-                scores<N, false>(p, x[q], unused);
-#pragma unroll
-                for (int i = 0; i < N; ++i) acc[i] += x[q][i];
+                for (int i = 0; i < N; ++i) x[i] = -INFINITY;
             }
+            scores<N, false>(p, x, unused);
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[i] += x[i];
         }
         // the warp's rows, then the warps, in a fixed order
         for (int o = 16; o >= p.lpr; o >>= 1)
@@ -250,7 +239,8 @@ __global__ void __launch_bounds__(kThreads, V * J <= 8 ? 4 : 1) balance_partial_
 
 // One cluster: CTA r owns the experts [r * cw, (r + 1) * cw).  A thread is (expert column, part): `per` parts share the
 // records of a sequence, parts / per sequences make a round (all powers of two).
-__global__ void __cluster_dims__(kFinishCtas, 1, 1) __launch_bounds__(kFinishThreads) balance_finish_kernel(const Params p, int cw, int parts, int per) {
+__global__ void __cluster_dims__(kFinishCtas, 1, 1) __launch_bounds__(kFinishThreads) balance_finish_kernel(const Params p) {
+    const int cw = p.cw, parts = p.parts, per = p.per;
     __shared__ float sP[kFinishThreads];
     __shared__ int sC[kFinishThreads], sN[kFinishThreads];
     __shared__ float total;
@@ -365,7 +355,7 @@ __device__ __forceinline__ void grad_row(const Params& p, int row, int sub, bool
 }
 
 template <int DT, int V, int J>
-__global__ void __launch_bounds__(kThreads, V * J <= 8 ? 3 : 1) balance_grad_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads) balance_grad_kernel(const Params p) {
     constexpr int N = V * J;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, sub = lane & (p.lpr - 1);
     const int rows_per_warp = 32 / p.lpr, group = lane / p.lpr, step = (kThreads / 32) * rows_per_warp;
@@ -386,43 +376,38 @@ __global__ void __launch_bounds__(kThreads, V * J <= 8 ? 3 : 1) balance_grad_ker
             const int c = column<V>(i, sub, p.lpr);
             u[i] = inside && c < p.E ? p.u[(long long)b * p.E + c] : 0.f;
         }
-        constexpr int RB = rows_at_once(N);
-        for (int r0 = a + warp * rows_per_warp + group; r0 - group < z; r0 += RB * step) {
-            float x[RB][N];
-            bool live[RB];
+        for (int r0 = a + warp * rows_per_warp; r0 < z; r0 += step) {
+            const int row = r0 + group;
+            bool live = inside && row < z;
+            float x[N];
+            load_row<DT, V, J>(p, row, sub, live, x);
+            if (p.mask != nullptr && live) live = p.mask[row] != 0;
+            if (!live)
 #pragma unroll
-            for (int q = 0; q < RB; ++q) {
-                const int row = r0 + q * step;
-                live[q] = inside && row < z;
-                load_row<DT, V, J>(p, row, sub, live[q], x[q]);
-                if (p.mask != nullptr && live[q]) live[q] = p.mask[row] != 0;
-            }
-#pragma unroll
-            for (int q = 0; q < RB; ++q)
-                if (!live[q])
-#pragma unroll
-                    for (int i = 0; i < N; ++i) x[q][i] = -INFINITY;
-#pragma unroll
-            for (int q = 0; q < RB; ++q) {
-                const int row = r0 + q * step;
-                grad_row<DT, V, J>(p, row < z ? row : -1, sub, live[q], g, x[q], u);
-            }
+                for (int i = 0; i < N; ++i) x[i] = -INFINITY;
+            grad_row<DT, V, J>(p, row < z ? row : -1, sub, live, g, x, u);
         }
         a = z;
     }
 }
 
-// A small batch in one CTA: scores in shared memory, sums per (sequence, expert) in token order split over a fixed number
-// of parts, then u, the loss, and the gradient if it is wanted.
+// A small batch in one launch, by one CTA or a cluster of eight that share the tokens: scores in shared memory, counts and
+// sums of p per (sequence, expert) of the own tokens, then, over the cluster in rank order, u, the loss and the counts, and
+// the gradient of the own tokens if it is wanted.
 template <int DT, int V, int J>
 __global__ void __launch_bounds__(kSmallThreads) balance_small_kernel(const Params p) {
     constexpr int N = V * J;
     extern __shared__ __align__(16) uint8_t smem[];
     const int sums = p.B * p.E;
-    float* const sp = reinterpret_cast<float*>(smem);                       // [T][E]
-    float* const su = sp + (size_t)p.T * p.E;                               // [B][E]
-    int* const sc = reinterpret_cast<int*>(su + sums);                      // [B][E]
-    int* const sn = sc + sums;                                              // [B]
+    int CL, rank;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(CL));
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    const int t0 = (int)((long long)p.T * rank / CL), t1 = (int)((long long)p.T * (rank + 1) / CL);
+    int* const sc = reinterpret_cast<int*>(smem);                           // [B][E] counts of the own tokens
+    float* const sP = reinterpret_cast<float*>(sc + sums);                  // [B][E] sums of p of the own tokens
+    float* const su = sP + sums;                                            // [B][E] u
+    int* const sn = reinterpret_cast<int*>(su + sums);                      // [B] own tokens counted
+    float* const sp = reinterpret_cast<float*>(sn + p.B);                   // [own tokens][E] scores
     __shared__ float red[kSmallThreads];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, sub = lane & (p.lpr - 1);
     const int rows_per_warp = 32 / p.lpr, group = lane / p.lpr, step = (kSmallThreads / 32) * rows_per_warp;
@@ -431,88 +416,114 @@ __global__ void __launch_bounds__(kSmallThreads) balance_small_kernel(const Para
     pdl_wait();
     pdl_launch_dependents();
     __syncthreads();
-    // sequence of a row, and whether the row is counted
-    auto live_of = [&](int row, int& b) {
-        if (row >= p.T) return false;
-        if (p.cu != nullptr) {
-            int lo = 0, hi = p.B;                                           // first sequence that ends behind the row
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (seq_start(p, mid + 1) > row) hi = mid;
-                else lo = mid + 1;
-            }
-            b = lo;
+    // sequence of a row (-1: none)
+    auto seq_of = [&](int row) {
+        if (p.cu == nullptr) return 0;
+        int lo = 0, hi = p.B;                                               // first sequence that ends behind the row
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (seq_start(p, mid + 1) > row) hi = mid;
+            else lo = mid + 1;
         }
-        return b < p.B && seq_start(p, b) <= row && (p.mask == nullptr || p.mask[row] != 0);
+        return lo < p.B && seq_start(p, lo) <= row ? lo : -1;
     };
-    int b = 0;
-    for (int r0 = warp * rows_per_warp; r0 < p.T; r0 += step) {
+    for (int r0 = t0 + warp * rows_per_warp; r0 < t1; r0 += step) {
         const int row = r0 + group;
-        const bool live = live_of(row, b);
         float x[N], unused[1];
-        load_row<DT, V, J>(p, row, sub, live, x);
-        if (live) {
+        load_row<DT, V, J>(p, row, sub, row < t1, x);
+        const int b = row < t1 && (p.mask == nullptr || p.mask[row] != 0) ? seq_of(row) : -1;
+        if (b >= 0) {
             for (int j = sub; j < p.topk; j += p.lpr) {
                 const int e = p.ids[(long long)row * p.topk + j];
                 if (e >= 0 && e < p.E) atomicAdd(&sc[b * p.E + e], 1);
             }
             if (sub == 0) atomicAdd(&sn[b], 1);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[i] = -INFINITY;
         }
         scores<N, false>(p, x, unused);
-        if (row < p.T)
+        if (row < t1)
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const int c = column<V>(i, sub, p.lpr);
-                if (c < p.E) sp[row * p.E + c] = x[i];
+                if (c < p.E) sp[(row - t0) * p.E + c] = x[i];
             }
     }
     __syncthreads();
-    // sums of p: thread = (pair, part); the parts of a pair are neighbours in `red`
+    // sums of p: thread = (pair, part); the parts of a pair are neighbours in a warp
     int parts = 1;
     while (parts * 2 * sums <= kSmallThreads && parts < 32) parts *= 2;
     const int pairs = kSmallThreads / parts;                                // pairs of one round
-    float loss = 0.f;
     for (int q0 = 0; q0 < sums; q0 += pairs) {
         const int q = q0 + tid / parts, sub_part = tid % parts;
         float P = 0.f;
         if (q < sums) {
-            const int sb = q / p.E, e = q - sb * p.E, s0 = seq_start(p, sb), s1 = seq_start(p, sb + 1);
-            for (int t = s0 + sub_part; t < s1; t += parts) P += sp[t * p.E + e];
+            const int sb = q / p.E, e = q - sb * p.E, s0 = max(seq_start(p, sb), t0), s1 = min(seq_start(p, sb + 1), t1);
+            for (int t = s0 + sub_part; t < s1; t += parts) P += sp[(t - t0) * p.E + e];
         }
         for (int h = parts >> 1; h > 0; h >>= 1) P += __shfl_xor_sync(0xFFFFFFFFu, P, h);
-        if (q < sums && sub_part == 0) {
-            const int sb = q / p.E, n = sn[sb];
-            const float u = n > 0 ? p.coef * (float)p.E * (float)sc[q] / ((float)p.B * (float)p.topk * (float)n * (float)n) : 0.f;
-            su[q] = u;
+        if (q < sums && sub_part == 0) sP[q] = P;
+    }
+    __syncthreads();
+    if (CL > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    auto over_cluster = [&](const void* at, auto zero) {
+        using T = decltype(zero);
+        if (CL == 1) return *reinterpret_cast<const T*>(at);
+        T v[kSmallCluster];                                                 // all on their way at once: a remote load takes 0.3 us
+#pragma unroll
+        for (int r = 0; r < kSmallCluster; ++r) {
+            uint32_t a, w;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(at)), "r"(r));
+            asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(w) : "r"(a) : "memory");
+            if constexpr (std::is_same<T, float>::value) v[r] = __uint_as_float(w);
+            else v[r] = (T)w;
+        }
+        T t = v[0];
+#pragma unroll
+        for (int r = 1; r < kSmallCluster; ++r) t += v[r];
+        return t;
+    };
+    float loss = 0.f;
+    for (int q = tid; q < sums; q += kSmallThreads) {
+        const int n = over_cluster(sn + q / p.E, 0), C = over_cluster(sc + q, 0);
+        const float u = n > 0 ? p.coef * (float)p.E * (float)C / ((float)p.B * (float)p.topk * (float)n * (float)n) : 0.f;
+        su[q] = u;
+        if (rank == 0) {
+            loss += u * over_cluster(sP + q, 0.f);
             if (p.u) p.u[q] = u;
-            loss += u * P;
         }
     }
-    red[tid] = loss;
-    __syncthreads();
-    for (int h = kSmallThreads / 2; h > 0; h >>= 1) {
-        if (tid < h) red[tid] += red[tid + h];
+    if (rank == 0) {
+        red[tid] = loss;
         __syncthreads();
+        for (int h = kSmallThreads / 2; h > 0; h >>= 1) {
+            if (tid < h) red[tid] += red[tid + h];
+            __syncthreads();
+        }
+        if (tid == 0) p.loss[0] = red[0];
+        for (int e = tid; e < p.E; e += kSmallThreads) {
+            int c = 0;
+            for (int q = 0; q < p.B; ++q) c += over_cluster(sc + q * p.E + e, 0);
+            p.counts[e] = c;
+        }
     }
-    if (tid == 0) p.loss[0] = red[0];
-    for (int e = tid; e < p.E; e += kSmallThreads) {
-        int c = 0;
-        for (int q = 0; q < p.B; ++q) c += sc[q * p.E + e];
-        p.counts[e] = c;
-    }
+    __syncthreads();
+    // nobody leaves, or writes its sums, while they may still be read
+    if (CL > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     if (p.grad == nullptr) return;
-    b = 0;
-    for (int r0 = warp * rows_per_warp; r0 < p.T; r0 += step) {
+    for (int r0 = t0 + warp * rows_per_warp; r0 < t1; r0 += step) {
         const int row = r0 + group;
-        const bool live = live_of(row, b);
         float x[N], u[N];
-        load_row<DT, V, J>(p, row, sub, live, x);
+        load_row<DT, V, J>(p, row, sub, row < t1, x);
+        const int b = row < t1 && (p.mask == nullptr || p.mask[row] != 0) ? seq_of(row) : -1;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int c = column<V>(i, sub, p.lpr);
-            u[i] = live && c < p.E ? su[b * p.E + c] : 0.f;
+            u[i] = b >= 0 && c < p.E ? su[b * p.E + c] : 0.f;
+            if (b < 0) x[i] = -INFINITY;
         }
-        grad_row<DT, V, J>(p, row < p.T ? row : -1, sub, live, 1.f, x, u);
+        grad_row<DT, V, J>(p, row < t1 ? row : -1, sub, b >= 0, 1.f, x, u);
     }
 }
 
@@ -545,10 +556,9 @@ Plan plan(int T, int E, int elem, bool aligned) {
     q.lpr = 1;
     while (q.lpr < 32 && q.lpr < vectors) q.lpr *= 2;
     q.j = (vectors + q.lpr - 1) / q.lpr;
-    // up to four runs per SM (a run with a sequence border in it takes two passes, and the launch waits for it), at least
-    // one pass of a block's warps each
-    const int rows = (kThreads / 32) * (32 / q.lpr) * rows_at_once(q.v * q.j);
-    const int want = 4 * sm_count();
+    // up to two runs per SM, at least one pass of a block's warps each
+    const int rows = (kThreads / 32) * (32 / q.lpr);
+    const int want = 2 * sm_count();
     q.R = std::max(rows, ((T + want - 1) / want + rows - 1) / rows * rows);
     q.runs = (T + q.R - 1) / q.R;
     return q;
@@ -573,17 +583,22 @@ Kern pick(int dt, int v, int j) {
     return dt == kF32 ? pick<kF32, KIND>(v, j) : (dt == kFP16 ? pick<kFP16, KIND>(v, j) : pick<kBF16, KIND>(v, j));
 }
 
-template <class K, class... A>
-int launch(const char* what, K kern, int grid, int threads, size_t smem, cudaStream_t s, A... args) {
+int launch(const char* what, Kern kern, int grid, int threads, size_t smem, cudaStream_t s, const Params& p, int cluster = 1) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute attr[2];
+    cudaLaunchAttribute attr[3];
     cfg.attrs = attr;
     cfg.numAttrs = launch_attrs(attr, 1);
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+    if (cluster > 1) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = (unsigned)cluster;
+        attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+        ++cfg.numAttrs;
+    }
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
     if (e != cudaSuccess) return fail(kCudaError, "%s launch: %s", what, cudaGetErrorString(e));
     return kOk;
 }
@@ -615,27 +630,34 @@ Plan plan_of(const BalanceParams& b) {
 
 }  // namespace
 
-// One CTA does the whole call: measured at 2048 x 8 and 96 x 128 (bf16), it takes 6 us where the three kernels take 9.
-static bool small_batch(int T, int E, int B) { return (long long)T * E <= kSmallElems && (long long)B * E <= kSmallSums && B <= 1024; }
+// CTAs of the one-launch form, 0 = the batch is too large for it.
+static int small_batch(int T, int E, int B) {
+    if ((long long)B * E > kSmallSums || B > 1024) return 0;
+    if ((long long)T * E <= kSmallElems / 8) return 1;
+    return (long long)((T + kSmallCluster - 1) / kSmallCluster) * E <= kSmallElems ? kSmallCluster : 0;
+}
 
 long long balance_workspace_bytes(int T, int E, int B) {
     if (T < 0 || E < 1 || B < 1 || small_batch(T, E, B)) return 0;
-    // the most runs any plan makes: 4 per SM, and never more than tokens
-    const long long records = (long long)std::min(T, 4 * sm_count() + 1) + B;
+    // the most runs any plan makes: 2 per SM, and never more than tokens
+    const long long records = (long long)std::min(T, 2 * sm_count() + 1) + B;
     return (records * E * 2 + records) * 4;
 }
 
 int launch_balance_loss(const BalanceParams& b, void* workspace, long long workspace_bytes, cudaStream_t s) {
     if (int st = check(b, "router_balance_loss")) return st;
-    const bool small = small_batch(b.T, b.E, b.B);
+    const int small = small_batch(b.T, b.E, b.B);
     if (!b.loss || !b.counts || (b.T > 0 && !b.ids)) return fail(kInvalidArg, "router_balance_loss: null pointer");
     if (!small && (!b.u || !workspace)) return fail(kInvalidArg, "router_balance_loss: null pointer (dprob, workspace)");
     const Plan q = plan_of(b);
     Params p = params(b, q);
     if (small) {
-        const size_t smem = ((size_t)b.T * b.E + 2 * (size_t)b.B * b.E + b.B) * 4;
+        const size_t most = (kSmallElems + 3 * kSmallSums + 1024) * 4;
         const Kern kern = pick<kSmall>(b.dtype, q.v, q.j);
-        return launch("router_balance_loss", kern, 1, kSmallThreads, smem, s, p);
+        if (umma::prepare_kernel(reinterpret_cast<const void*>(kern), kSmallThreads, most, 0) == 0)
+            return fail(kCudaError, "router_balance_loss: the kernel cannot be launched on this device");
+        const size_t rows = (b.T + small - 1) / small;
+        return launch("router_balance_loss", kern, small, kSmallThreads, (rows * b.E + 3 * (size_t)b.B * b.E + b.B) * 4, s, p, small);
     }
     const long long records = (long long)q.runs + b.B;
     if (workspace_bytes < (records * b.E * 2 + records) * 4)
@@ -645,13 +667,17 @@ int launch_balance_loss(const BalanceParams& b, void* workspace, long long works
     p.N = p.C + records * b.E;
     if (b.T > 0) {
         const size_t smem = (size_t)(kThreads / 32 + 1) * b.E * 4;
-        if (int st = launch("router_balance_loss", pick<kPartial>(b.dtype, q.v, q.j), q.runs, kThreads, smem, s, p)) return st;
+        const Kern kern = pick<kPartial>(b.dtype, q.v, q.j);
+        if (smem > 40 * 1024 && umma::prepare_kernel(reinterpret_cast<const void*>(kern), kThreads, (kThreads / 32 + 1) * kBalanceMaxExperts * 4, 0) == 0)
+            return fail(kCudaError, "router_balance_loss: the kernel cannot be launched on this device");
+        if (int st = launch("router_balance_loss", kern, q.runs, kThreads, smem, s, p)) return st;
     }
     const int cw = (b.E + kFinishCtas - 1) / kFinishCtas;
     int parts = 1, per = 1;
     while (parts * 2 * cw <= kFinishThreads) parts *= 2;
     while (per * 2 <= parts && per * 2 * b.B <= parts) per *= 2;
-    if (int st = launch("router_balance_loss (finish)", balance_finish_kernel, kFinishCtas, kFinishThreads, 0, s, p, cw, parts, per)) return st;
+    p.cw = cw; p.parts = parts; p.per = per;
+    if (int st = launch("router_balance_loss (finish)", balance_finish_kernel, kFinishCtas, kFinishThreads, 0, s, p)) return st;
     return b.grad ? launch_balance_grad(b, s) : (int)kOk;
 }
 
@@ -671,8 +697,17 @@ int launch_expert_counts(const int32_t* ids, const uint8_t* mask, int T, int top
     if (e != cudaSuccess) return fail(kCudaError, "expert_counts: %s", cudaGetErrorString(e));
     if (T == 0) return kOk;
     const long long n = (long long)T * topk;
-    const int grid = (int)std::min<long long>((n + 4 * kThreads - 1) / (4 * kThreads), 2LL * sm_count());
-    return launch("expert_counts", expert_counts_kernel, grid, kThreads, (size_t)E * 4, s, ids, mask, n, topk, E, counts);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)std::min<long long>((n + 4 * kThreads - 1) / (4 * kThreads), 2LL * sm_count()));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = (size_t)E * 4;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    cfg.attrs = attr;
+    cfg.numAttrs = launch_attrs(attr, 1);
+    e = cudaLaunchKernelEx(&cfg, expert_counts_kernel, ids, mask, n, topk, E, counts);
+    if (e != cudaSuccess) return fail(kCudaError, "expert_counts launch: %s", cudaGetErrorString(e));
+    return kOk;
 }
 
 }  // namespace mlk

@@ -107,6 +107,29 @@ int launch_w4_experts(const W4ExpertsParams& p, cudaStream_t s) {
     void* const act = ws + l.act;
     float* const scratch = reinterpret_cast<float*>(ws + l.scratch);
 
+    W4KernelParams g{};
+    g.topk_weights = p.topk_weights;
+    g.topk = p.topk;
+    if (p.T == 1 && p.topk <= 8) {
+        // a single token: its slots are the work items, and a cluster of them sums the result: two launches, no work list
+        g.ids = p.topk_ids;
+        g.experts_map = p.experts_map;
+        g.experts_map_len = p.experts_map_len;
+        g.experts = p.E;
+        g.y_fp32 = p.y_fp32;
+        g.X = p.x;
+        g.C = act;
+        g.k = p.H;
+        g.out_tiles = p.I / 16;
+        g.mat_tiles = 2 * p.I / 16;
+        if (int st = launch_w4_mma(1, p.dtype, g, p.w1, p.topk, p.topk, 1, s)) return st;
+        g.X = act;
+        g.C = p.y;
+        g.k = p.I;
+        g.out_tiles = g.mat_tiles = p.H / 16;
+        return launch_w4_mma(2, p.dtype, g, p.w2, p.topk, p.topk, 1, s);
+    }
+
     // Slots of a work item, by the slots an expert gets: the streaming kernel up to 4, above it tcgen05 with 32, 64 or 128.
     // Measured (us): 2 slots 63 against 81, 4 slots 82 / 174 against 98 / 176, 8 slots 130 / 230 against 109 / 186 (128 experts of
     // 2048 x 768 / 8 of 4096 x 14336); 32 against 64 slots a tile: 127 / 190 against 142 / 215 at 16 slots, 173 / 273
@@ -121,11 +144,8 @@ int launch_w4_experts(const W4ExpertsParams& p, cudaStream_t s) {
                                   p.experts_map, p.experts_map_len, s, worklist, block))
         return st;
 
-    W4KernelParams g{};
     g.worklist = worklist;
     g.sorted = sorted;
-    g.topk_weights = p.topk_weights;
-    g.topk = p.topk;
     g.X = p.x;
     g.C = act;
     g.k = p.H;

@@ -23,6 +23,12 @@ struct W4KernelParams {
     const int32_t* sorted;      // slot id of every position
     const void* topk_weights;
     int topk;
+    // a single token: work item = slot, no work list.  The first product leaves row `slot` of the activation; the CTAs of a
+    // cluster of the second are the token's slots, and their weighted sum is the result.
+    const int32_t* ids;         // [topk], or null
+    const int32_t* experts_map;
+    int experts_map_len, experts;
+    int y_fp32;
 };
 
 template <int WT>
@@ -42,6 +48,7 @@ struct W4UmmaPlan {
     double us;                  // estimated time
 };
 W4UmmaPlan w4_umma_plan(int rows16, int n, int k);
+// With p.ids the experts' modes take a single token's slots (at most 8) as their items.
 int launch_w4_mma(int mode, int wt, W4KernelParams p, const W4Weights& w, int items, int likely_items, int nt, cudaStream_t s);
 
 }  // namespace mlk

@@ -69,6 +69,13 @@ __device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4],
 
 constexpr int kWarps = 8, kRT = 4, kDI = 2;     // warps of a CTA, row tiles of a warp, ring depth in units
 
+// Local expert of a slot of the single token, -1 = none here.
+__device__ __forceinline__ int expert_of(const W4KernelParams& p, int slot) {
+    int e = p.ids[slot];
+    if (p.experts_map != nullptr) e = e >= 0 && e < p.experts_map_len ? p.experts_map[e] : -1;
+    return e >= 0 && e < p.experts ? e : -1;
+}
+
 // NT: column tiles of 8 tokens; RT: 16-row tiles of a warp (MODE 1: half gate, half up); DI: ring depth in units of 128 k;
 // G: group size; ZP: zero points given.
 template <int WT, int NT, int RT, int DI, int G, bool ZP, int MODE>
@@ -79,7 +86,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) w4_mma_kernel(co
     constexpr int NG = 128 / G, SG = G / 16;             // groups of a unit, 16-k steps of a group
     constexpr uint32_t kSlot = RT * 2 * kW4BlockBytes;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, t = lane & 3;
+    const bool single = MODE != 0 && p.ids != nullptr;   // one token: items are its slots
+    const bool gathered = MODE == 2 && single;           // the cluster's CTAs are the slots, not parts of k
     const int rank = blockIdx.y, SK = gridDim.y;
+    const int krank = gathered ? 0 : rank, KSK = gathered ? 1 : SK;
     const int WR = p.row_warps, WK = kWarps / WR, wr = warp / WK, wk = warp - wr * WK;
     const int tile0 = blockIdx.x * RO * WR;
 
@@ -93,6 +103,14 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) w4_mma_kernel(co
     if constexpr (MODE == 0) {
         n0 = blockIdx.z * NT * 8;
         ntok = min(NT * 8, p.n - n0);
+    } else if (single) {
+        cpos0 = gathered ? rank : blockIdx.z;            // the slot
+        mat = expert_of(p, cpos0);
+        ntok = 1;
+        if (mat < 0) {
+            if (!gathered) return;                       // uniform over the cluster: its row is not read either
+            mat = ntok = 0;                              // nothing of this slot: zeros for the sum
+        }
     } else {
         const int items = p.worklist[0].x;
         const int4 item = p.worklist[1 + blockIdx.z];
@@ -106,7 +124,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) w4_mma_kernel(co
         return MODE == 1 && j >= RO ? tile + p.out_tiles : tile;
     };
     const int units = (p.kc + 1) >> 1;                   // two blocks (128 k) each; the last one of an odd number is half
-    const int ub = (int)((long long)units * rank / SK), ue = (int)((long long)units * (rank + 1) / SK);
+    const int ub = (int)((long long)units * krank / KSK), ue = ntok == 0 ? ub : (int)((long long)units * (krank + 1) / KSK);
     const size_t tile_bytes = (size_t)p.kc * kW4BlockBytes;
     const uint8_t* wnext[RT];                            // the unit that is fetched next
 #pragma unroll
@@ -148,7 +166,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) w4_mma_kernel(co
             if (in) {
                 long long row;
                 if constexpr (MODE == 0) row = n0 + c;
-                else if constexpr (MODE == 1) row = p.sorted[pos0 + c] / p.topk;
+                else if constexpr (MODE == 1) row = single ? 0 : p.sorted[pos0 + c] / p.topk;
                 else row = cpos0 + c;
                 src += (row * p.k + k0) * 2 + o * 16;
             }
@@ -271,36 +289,52 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) w4_mma_kernel(co
         for (int q = 1; q < WK; ++q) add(v, *reinterpret_cast<const float4*>(red + q * kPerWarp + at));
         return v;
     };
-    if (SK > 1) {
+    const int cols = gathered ? 1 : ntok;                // a skipped slot of a single token adds zeros
+    if (SK > 1 || gathered) {
         if (WK > 1) {
-            for (int e = tid; e < WR * RT * 4 * ntok; e += kWarps * 32) {
+            for (int e = tid; e < WR * RT * 4 * cols; e += kWarps * 32) {
                 const int q = e & 3, i = (e >> 2) % RT, rest = (e >> 2) / RT, w = rest % WR, tok = rest / WR;
                 const int at = place(w, i, tok, q);
                 *reinterpret_cast<float4*>(red + at) = warps_sum(at);
             }
         }
         __syncwarp();
-        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (SK > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        else __syncthreads();
     }
+    auto part = [&](int q, int at) {                     // rank q's sums
+        if (SK == 1) return *reinterpret_cast<const float4*>(red + at);
+        uint32_t a;
+        float4 o;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem0 + 4u * at), "r"(q));
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(o.x), "=f"(o.y), "=f"(o.z), "=f"(o.w) : "r"(a) : "memory");
+        return o;
+    };
     auto total = [&](int at) {
         if (SK == 1) return warps_sum(at);
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int q = 0; q < SK; ++q) {
-            uint32_t a;
-            float4 o;
-            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem0 + 4u * at), "r"(q));
-            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(o.x), "=f"(o.y), "=f"(o.z), "=f"(o.w) : "r"(a) : "memory");
-            add(v, o);
-        }
+        for (int q = 0; q < SK; ++q) add(v, part(q, at));
         return v;
     };
-    const int outs = WR * RO * 4 * ntok;
+    const int outs = WR * RO * 4 * cols;
     const size_t ld = (size_t)p.out_tiles * 16;
     for (int e = outs * rank / SK + tid; e < outs * (rank + 1) / SK; e += kWarps * 32) {
         const int q = e & 3, i = (e >> 2) % RO, rest = (e >> 2) / RO, w = rest % WR, tok = rest / WR;
         const int tile = tile0 + w * RO + i;
         if (tile >= p.out_tiles) continue;
         const int row = tile * 16 + 4 * q;
+        if (MODE == 2 && single) {
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);  // the token's slots in order, in fp32, rounded once
+            for (int j = 0; j < SK; ++j) {
+                if (expert_of(p, j) < 0) continue;
+                const float f = load_scalar16<WT>(p.topk_weights, j);
+                const float4 v = part(j, place(w, i, tok, q));
+                y.x += f * v.x; y.y += f * v.y; y.z += f * v.z; y.w += f * v.w;
+            }
+            if (p.y_fp32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.C) + row) = y;
+            else *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.C) + row) = make_uint2(pack2<WT>(y.x, y.y), pack2<WT>(y.z, y.w));
+            continue;
+        }
         const float4 v = total(place(w, i, tok, q));
         if constexpr (MODE == 0) {
             float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -374,17 +408,19 @@ struct Plan {
 // to start, stage and reduce; a CTA alone on an SM takes 0.95 us for an iteration of its warps (32 KB of weights) with 8
 // tokens, 2.0 with 16; several on an SM share the memory at 0.87 and 1.1 us per CTA; and rounds are whole.  (Fitted to
 // sweeps over 4096 x 4096 .. 28672 x 8192 and the expert shapes; the best and the chosen split differ by at most 8 % there.)
-Plan make_plan(const void* kern, int mode, int nt, int group, bool zp, int tiles, int units, int items) {
+// `slots` > 0: the cluster is that many CTAs, each over the whole k (the second product of a single token).
+Plan make_plan(const void* kern, int mode, int nt, int group, bool zp, int tiles, int units, int items, int slots) {
     Plan best{1, 1, 1, 0};
     double best_us = 1e30;
     const size_t ring = (size_t)kWarps * kDI * kRT * 1024;
     for (int wr = 1; wr <= kWarps; wr *= 2)
-        for (int sk = 1; sk <= 8 && sk <= units; ++sk) {
+        for (int sk = slots > 0 ? slots : 1; sk <= (slots > 0 ? slots : std::min(8, units)); ++sk) {
             const int ro = (mode == 1 ? kRT / 2 : kRT) * wr, wk = kWarps / wr;
             if (wr > 1 && ro / 2 >= tiles) continue;                    // half of the row warps would have nothing to do
             auto staged = [&](int n) { return (size_t)nt * 8 * (n * 256 + 32) + (size_t)wr * kRT * n * (128 / group) * (zp ? 48 : 32); };
             // a segment: the CTA's whole k range where it fits beside the ring, else as many units as do
-            int seg = (units + sk - 1) / sk;
+            const int per_rank = slots > 0 ? units : (units + sk - 1) / sk;
+            int seg = per_rank;
             while (ring + staged(seg) > 200 * 1024) seg = (seg + 1) / 2;
             const size_t smem = std::max(ring + staged(seg), (size_t)kWarps * kRT * nt * 8 * kTokStride * 4);
             int resident = 0;
@@ -392,7 +428,6 @@ Plan make_plan(const void* kern, int mode, int nt, int group, bool zp, int tiles
             if (launch_smem == 0) continue;
             const int room = active_clusters(kern, launch_smem, sk, resident);
             if (room < 1) continue;
-            const int per_rank = (units + sk - 1) / sk;
             const double clusters = (double)((tiles + ro - 1) / ro) * items, iters = (per_rank + wk - 1) / wk;
             const double rounds = std::ceil(clusters / room), share = std::min<double>(resident, std::ceil(clusters * sk / sm_count()));
             const double iter_us = nt == 1 ? std::max(0.95, 0.87 * share) : std::max(2.0, 1.1 * share);
@@ -405,17 +440,17 @@ Plan make_plan(const void* kern, int mode, int nt, int group, bool zp, int tiles
     return best;
 }
 
-Plan cached_plan(const void* kern, int mode, int nt, int group, bool zp, int tiles, int units, int items) {
+Plan cached_plan(const void* kern, int mode, int nt, int group, bool zp, int tiles, int units, int items, int slots) {
     static std::mutex mu;
     static std::map<std::array<long long, 6>, Plan> known;
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return Plan{1, 1, 1, 0};
-    const std::array<long long, 6> key{(long long)(uintptr_t)kern, dev, tiles, units, items, 0};
+    const std::array<long long, 6> key{(long long)(uintptr_t)kern, dev, tiles, units, items, slots};
     std::lock_guard<std::mutex> lock(mu);
     auto it = known.find(key);
     if (it != known.end()) return it->second;
     if (known.size() > 4096) known.clear();              // a server sees a few hundred shapes
-    return known[key] = make_plan(kern, mode, nt, group, zp, tiles, units, items);
+    return known[key] = make_plan(kern, mode, nt, group, zp, tiles, units, items, slots);
 }
 
 }  // namespace
@@ -430,14 +465,15 @@ int launch_w4_mma(int mode, int wt, W4KernelParams p, const W4Weights& w, int it
     if (items > 65535) return fail(kUnsupported, "w4: %d work items exceed one launch", items);
     const void* kern = wt == kFP16 ? pick<kFP16>(mode, nt, w.group, zp) : pick<kBF16>(mode, nt, w.group, zp);
     if (kern == nullptr) return fail(kInvalidArg, "w4: %d tokens per item are not built", 8 * nt);
-    const Plan q = cached_plan(kern, mode, nt, w.group, zp, p.out_tiles, (p.kc + 1) / 2, likely_items);
+    const Plan q = cached_plan(kern, mode, nt, w.group, zp, p.out_tiles, (p.kc + 1) / 2, mode == 2 && p.ids ? 1 : likely_items,
+                               mode == 2 && p.ids ? p.topk : 0);
     if (q.smem == 0) return fail(kCudaError, "w4: the streaming kernel cannot be launched on this device");
     p.seg_units = q.seg;
     p.row_warps = q.wr;
     const int ro = (mode == 1 ? kRT / 2 : kRT) * q.wr;
     int static_weights = option(kOptStaticWeights);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((p.out_tiles + ro - 1) / ro), (unsigned)q.sk, (unsigned)items);
+    cfg.gridDim = dim3((unsigned)((p.out_tiles + ro - 1) / ro), (unsigned)q.sk, (unsigned)(mode == 2 && p.ids ? 1 : items));
     cfg.blockDim = dim3(kWarps * 32);
     cfg.dynamicSmemBytes = q.smem;
     cfg.stream = s;

@@ -197,7 +197,7 @@ def fused_experts_compute_w4(w1, w1_scales, w2, w2_scales, activations, topk_ids
     dtype = x.dtype if out_dtype is None else out_dtype
     _chk(dtype is x.dtype or dtype is torch.float32, "out_dtype must be the activation data type or torch.float32")
     if out is None:
-        out = x.new_empty((T, H), dtype=dtype)
+        out = torch.empty_like(x) if dtype is x.dtype else x.new_empty((T, H), dtype=dtype)
     else:
         _chk(out.get_device() == d and out.is_contiguous() and out.shape == x.shape and out.dtype is dtype,
              "out must be a contiguous [T, H] in the result's data type on the activations' device")

@@ -55,7 +55,7 @@ def test_c_entry_refuses_bad_arguments():
     ok = 1 << 20                                  # an aligned address that no refused call reads
 
     def loss(**kw):
-        a = dict(logits=ok, ids=ok, mask=None, cu=None, T=5000, E=8, topk=2, B=1, score=0, coef=1.0, dtype=0, loss=ok, counts=ok,
+        a = dict(logits=ok, ids=ok, mask=None, cu=None, T=50000, E=8, topk=2, B=1, score=0, coef=1.0, dtype=0, loss=ok, counts=ok,
                  dprob=ok, grad=None, ws=ok, nbytes=1 << 20)
         a.update(kw)
         return lib.mlk_router_balance_loss(*a.values(), None)
