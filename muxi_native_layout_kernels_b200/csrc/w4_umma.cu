@@ -99,8 +99,9 @@ __global__ void __launch_bounds__(kThreads, tmem_columns(MODE == 1 ? 2 : 1, NP) 
     __shared__ __align__(8) uint64_t bars[2 * RS + 2 * S2 + 2 * SB + 2];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int abort_flag;
-    // MODE 2: slot and routing weight of every token of the item (fetched where they are used, each column of the read-out
-    // waited for two dependent loads behind the stores of the one before: 10 us for 16 columns)
+    // MODE 2: slot and routing weight of every token of the item.  (Fetched where they are used, each column of the read-out
+    // waits for two dependent loads behind the stores of the one before: 181 instead of 153 us for 512 tokens x 8 on 128
+    // experts of 2048 x 768, both products.)
     __shared__ int slot_of[MODE == 2 ? NP : 1];
     __shared__ float weight_of[MODE == 2 ? NP : 1];
 
@@ -109,11 +110,8 @@ __global__ void __launch_bounds__(kThreads, tmem_columns(MODE == 1 ? 2 : 1, NP) 
     const int row_tiles = (p.out_tiles + 7) / 8, tile = blockIdx.x * u.run, rank = blockIdx.y, SK = gridDim.y;
     const int run = min(u.run, row_tiles - tile);
 
-    const bool early = MODE == 0 && static_weights;
-    if (!early) {
-        pdl_wait();
-        pdl_launch_dependents();
-    }
+    const bool early = MODE == 0 && static_weights;  // weights may be fetched before the kernel in front has finished
+    if (!early) pdl_wait();
     int mat = 0, pos0 = 0, row0 = 0, ntok;       // row0: first row of the token tile
     if constexpr (MODE == 0) {
         row0 = blockIdx.z * NP;
@@ -164,6 +162,39 @@ __global__ void __launch_bounds__(kThreads, tmem_columns(MODE == 1 ? 2 : 1, NP) 
         abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+
+    const int g16 = mat * p.mat_tiles + tile * 8;                      // first 16-row group
+    auto load_raw = [&](int i, int t, int s) {   // stage i of row tile t of the run
+        const uint64_t wpol = l2_evict_first_policy();
+        if (elect_one()) {
+            mbar_expect_tx(raw_full(s), NA * kTile);
+#pragma unroll
+            for (int w = 0; w < NA; ++w) {
+                const uint32_t dst = r_base + (s * NA + w) * kTile;
+                const int g = g16 + t * 8 + (w == 1 ? p.out_tiles : 0);
+                tma_load_3d_hint(dst, &map_q, raw_full(s), 0, (st0 + i) * 2, g, wpol);
+                tma_load_3d(dst + kRaw, &map_s, raw_full(s), 0, (st0 + i) * NG, g);
+                if constexpr (ZP) tma_load_3d(dst + kRaw + 256 * NG, &map_z, raw_full(s), 0, (st0 + i) * NG, g);
+            }
+        }
+        __syncwarp();
+    };
+    int ri = 0, rs = 0, rk = 0, rt = 0;          // the producer's next raw stage, its ring slot, and as (stage, row tile)
+    uint32_t rpar = 1;                           // parity that says the slot is free: the first round finds it so
+    if (early) {
+        if (warp == 0) {
+            __syncwarp();
+            for (; ri < min(total, RS); ++ri) {
+                load_raw(rk, rt, ri);
+                if (++rk == n) { rk = 0; ++rt; }
+            }
+            if (ri == RS) rpar ^= 1u;
+            rs = ri % RS;
+        }
+        pdl_wait();
+    }
+    // Tensor memory is taken when the kernel in front has finished, and the next kernel is let in when it has been: a CTA
+    // never holds columns while it waits for a kernel that may still be asking for them.
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
                      "r"(kTmemCols)
@@ -174,6 +205,7 @@ __global__ void __launch_bounds__(kThreads, tmem_columns(MODE == 1 ? 2 : 1, NP) 
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, tmem_slot, 0);
+    pdl_launch_dependents();
 
     // ---- read-out of one row tile where this CTA has the whole sums: set 0 the lower half of the tokens, set 1 the upper,
     // straight from tensor memory, a thread has one row, neighbouring lanes neighbouring rows ----
@@ -214,35 +246,8 @@ __global__ void __launch_bounds__(kThreads, tmem_columns(MODE == 1 ? 2 : 1, NP) 
     int raw_issued = 0, x_issued = 0;
     if (warp == 0) {
         // ---- TMA producer: raw weights and token tiles are two independent streams, polled without blocking ----
-        const uint64_t wpol = l2_evict_first_policy();
-        const int g16 = mat * p.mat_tiles + tile * 8;                  // first 16-row group
-        auto load_raw = [&](int i, int t, int s) {   // stage i of row tile t of the run
-            if (elect_one()) {
-                mbar_expect_tx(raw_full(s), NA * kTile);
-#pragma unroll
-                for (int w = 0; w < NA; ++w) {
-                    const uint32_t dst = r_base + (s * NA + w) * kTile;
-                    const int g = g16 + t * 8 + (w == 1 ? p.out_tiles : 0);
-                    tma_load_3d_hint(dst, &map_q, raw_full(s), 0, (st0 + i) * 2, g, wpol);
-                    tma_load_3d(dst + kRaw, &map_s, raw_full(s), 0, (st0 + i) * NG, g);
-                    if constexpr (ZP) tma_load_3d(dst + kRaw + 256 * NG, &map_z, raw_full(s), 0, (st0 + i) * NG, g);
-                }
-            }
-            __syncwarp();
-        };
-        int ri = 0, xi = 0, rs = 0, xs = 0;      // next stage of each stream and its ring slot
-        int rk = 0, rt = 0, xk = 0;              // the same as (stage, row tile)
-        uint32_t rpar = 1, xpar = 1;             // parity that says the slot is free: the first round finds it so
-        if (early) {
-            for (; ri < min(total, RS); ++ri) {
-                load_raw(rk, rt, ri);
-                if (++rk == n) { rk = 0; ++rt; }
-            }
-            if (ri == RS) rpar ^= 1u;
-            rs = ri % RS;
-            pdl_launch_dependents();
-            pdl_wait();
-        }
+        int xi = 0, xs = 0, xk = 0;              // the next token tile, its ring slot, its stage within a row tile
+        uint32_t xpar = 1;
         uint32_t idle = 0;
         while ((xi < total || ri < total) && !__any_sync(kAll, abort_flag)) {
             bool progressed = false;
@@ -279,7 +284,6 @@ __global__ void __launch_bounds__(kThreads, tmem_columns(MODE == 1 ? 2 : 1, NP) 
         x_issued = xi;
     } else if (warp == 1) {
         // ---- MMA issuer ----
-        if (early) pdl_wait();                   // the bounded waits must not count the kernel in front
         constexpr uint32_t idesc = instr_desc<WT, NP>();
         const uint64_t d0 = smem_desc(x_base, 16, 1024, 2);
         const uint32_t a0 = tmem + NA * NP;
@@ -317,7 +321,6 @@ __global__ void __launch_bounds__(kThreads, tmem_columns(MODE == 1 ? 2 : 1, NP) 
         }
     } else if (warp >= 2) {
         // ---- converter warps ----
-        if (early) pdl_wait();
         const int quad = warp & 3, set = (warp - 2) >> 2, r = lane >> 2;
         constexpr int kStep = NA == 2 ? 1 : 2;   // stages of a set
         int s = NA == 2 ? 0 : set, s2 = s % S2;
@@ -508,26 +511,31 @@ const void* pick(int mode, int np, int group, bool zp) {
     return nullptr;
 }
 
-// Tensor maps over 16-row groups: packed blocks [groups16][kc][128 words], scales [groups16][groups][16], zero points alike.
+// Tensor maps over 16-row groups: packed blocks [groups16][kc][128 words], scales [groups16][groups][16], zero points alike;
+// and over the token rows.  Encoded for every launch.
 bool map_packed(CUtensorMap* m, const void* q, long long groups16, int kc) {
-    return cached_map(m, 11, q, groups16, kc, 0, [&](CUtensorMap* t) {
-        const cuuint64_t dims[3] = {128, (cuuint64_t)kc, (cuuint64_t)groups16};
-        const cuuint64_t strides[2] = {kW4BlockBytes, (cuuint64_t)kc * kW4BlockBytes};
-        const cuuint32_t box[3] = {128, 2, 8}, estr[3] = {1, 1, 1};
-        return encode_fn()(t, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void*>(q), dims, strides, box, estr,
-                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-    });
+    const cuuint64_t dims[3] = {128, (cuuint64_t)kc, (cuuint64_t)groups16};
+    const cuuint64_t strides[2] = {kW4BlockBytes, (cuuint64_t)kc * kW4BlockBytes};
+    const cuuint32_t box[3] = {128, 2, 8}, estr[3] = {1, 1, 1};
+    return encode_fn()(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void*>(q), dims, strides, box, estr,
+                       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 bool map_groups(CUtensorMap* m, const void* v, long long groups16, int groups, int group, int elem) {
-    return cached_map(m, 12, v, groups16, groups, group * 4 + elem, [&](CUtensorMap* t) {
-        const cuuint64_t dims[3] = {16, (cuuint64_t)groups, (cuuint64_t)groups16};
-        const cuuint64_t strides[2] = {(cuuint64_t)16 * elem, (cuuint64_t)groups * 16 * elem};
-        const cuuint32_t box[3] = {16, (cuuint32_t)(kStageK / group), 8}, estr[3] = {1, 1, 1};
-        return encode_fn()(t, elem == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(v), dims,
-                           strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
-                           CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-    });
+    const cuuint64_t dims[3] = {16, (cuuint64_t)groups, (cuuint64_t)groups16};
+    const cuuint64_t strides[2] = {(cuuint64_t)16 * elem, (cuuint64_t)groups * 16 * elem};
+    const cuuint32_t box[3] = {16, (cuuint32_t)(kStageK / group), 8}, estr[3] = {1, 1, 1};
+    return encode_fn()(m, elem == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(v), dims,
+                       strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                       CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+bool map_tokens(CUtensorMap* m, const void* X, int n, int k, int wt, int np) {
+    const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)n};
+    const cuuint64_t strides[1] = {(cuuint64_t)k * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)np}, estr[2] = {1, 1};
+    return encode_fn()(m, wt == kFP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(X),
+                       dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                       CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // Estimated time (us) of a product: a CTA costs 5 us to start and to read out (1 more with a cluster), a stage of 128 k on an
@@ -587,7 +595,7 @@ int launch_w4_umma(int mode, int wt, const W4KernelParams& kp, const W4Weights& 
     } else {
         mz = ms;
     }
-    if (!make_map_x(&mx, kp.X, x_rows, kp.k, wt, np)) return fail(kUnsupported, "w4 (tcgen05): activation tensor map rejected");
+    if (!map_tokens(&mx, kp.X, x_rows, kp.k, wt, np)) return fail(kUnsupported, "w4 (tcgen05): activation tensor map rejected");
     const size_t tile = kRaw + 256 * ng + (zp ? 128 * ng : 0);
     const size_t rings = (size_t)token_stages(np) * np * 256 + (size_t)raw_stages(na) * na * tile;
     const size_t partial = sk > 1 ? (size_t)na * std::min(np, 64) * kTileM * 4 : 0;

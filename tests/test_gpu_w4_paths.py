@@ -97,6 +97,44 @@ def test_static_weights_option(n):
     assert mlk().kernel_status() == 0
 
 
+@pytest.mark.parametrize("captured", [False, True])
+def test_static_weights_in_a_chain(captured):
+    """Experts, then products of every kind, each the input of the next, with the weights fetched ahead."""
+    dev = require_gpu()
+    E, topk, H, I, T = 8, 2, 256, 128, 300
+    w1 = laid_out(ow4.random_weights(2 * I, H, 128, torch.bfloat16, 1, False, (E,)), dev)
+    w2 = laid_out(ow4.random_weights(H, I, 64, torch.bfloat16, 2, True, (E,)), dev)
+    d = laid_out(ow4.random_weights(H, H, 32, torch.bfloat16, 3, False), dev)
+    g = torch.Generator().manual_seed(5)
+    x = randn((T, H), 6, 1.0, torch.bfloat16).to(dev)
+    ids = torch.rand(T, E, generator=g).topk(topk, -1)[1].to(torch.int32).to(dev)
+    p = torch.rand(T, topk, generator=g).to(torch.bfloat16).to(dev)
+
+    def chain():
+        y = mlk().fused_experts_compute_w4(w1[0], w1[1], w2[0], w2[1], x, ids, p, w2_zeros=w2[2])
+        for n in (T, 250, 100, 60, 20, 16, 8, 1):
+            y = mlk().gemm_layoutA_w4(d[0], d[1], y[:n].contiguous(), alpha=0.25)
+            y = mlk().gemm_layoutA_w4(d[0], d[1], y, alpha=0.25)
+        return y
+
+    want = chain()
+    torch.cuda.synchronize()
+    mlk().set_static_weights(True)
+    try:
+        if captured:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                got = chain()
+            for _ in range(5):
+                graph.replay()
+        else:
+            for _ in range(5):
+                got = chain()
+        assert torch.equal(got, want) and mlk().kernel_status() == 0
+    finally:
+        mlk().set_static_weights(False)
+
+
 @pytest.mark.parametrize("T", [1, 7, 90])
 def test_two_graphs_at_once(T):
     """Two captured layers, replayed on two streams at the same time with inputs of their own."""
