@@ -611,6 +611,10 @@ int check(const BalanceParams& b, const char* who) {
     if (b.B > 1 && !b.cu_seqlens) return fail(kInvalidArg, "%s: more than one sequence needs cu_seqlens", who);
     if (b.T > 0 && !b.logits) return fail(kInvalidArg, "%s: null pointer", who);
     if ((long long)b.B + b.T > 0x3FFFFFFF) return fail(kUnsupported, "%s: too many tokens or sequences", who);
+    if ((long long)b.T * b.topk > 0x7FFFFFFF) return fail(kUnsupported, "%s: counts of more than 2^31 - 1 picks", who);
+    const uintptr_t elem = b.dtype == kF32 ? 3 : 1;
+    if ((((uintptr_t)b.logits | (uintptr_t)b.grad) & elem) || (((uintptr_t)b.ids | (uintptr_t)b.cu_seqlens) & 3))
+        return fail(kInvalidArg, "%s: logits, grad, topk_ids or cu_seqlens is not aligned", who);
     return kOk;
 }
 
@@ -692,7 +696,9 @@ int launch_balance_grad(const BalanceParams& b, cudaStream_t s) {
 int launch_expert_counts(const int32_t* ids, const uint8_t* mask, int T, int topk, int E, int32_t* counts, cudaStream_t s) {
     if (T < 0 || topk < 1) return fail(kInvalidArg, "expert_counts: bad sizes");
     if (E < 1 || E > kBalanceMaxExperts) return fail(kUnsupported, "expert_counts: 1 <= experts <= %d (got %d)", kBalanceMaxExperts, E);
+    if ((long long)T * topk > 0x7FFFFFFF) return fail(kUnsupported, "expert_counts: counts of more than 2^31 - 1 picks");
     if (!counts || (T > 0 && !ids)) return fail(kInvalidArg, "expert_counts: null pointer");
+    if ((uintptr_t)ids & 3) return fail(kInvalidArg, "expert_counts: topk_ids is not aligned");
     cudaError_t e = cudaMemsetAsync(counts, 0, (size_t)E * 4, s);
     if (e != cudaSuccess) return fail(kCudaError, "expert_counts: %s", cudaGetErrorString(e));
     if (T == 0) return kOk;

@@ -21,6 +21,7 @@ namespace mlk {
 
 constexpr int kW4BlockK = 64;        // k per 512-byte block
 constexpr int kW4BlockBytes = 512;
+constexpr int kW4MaxDim = 1 << 28;   // rows of a matrix and k: keeps 32-bit row and byte-in-row arithmetic exact
 
 struct W4Weights {
     const uint8_t* q;      // packed blocks
@@ -34,7 +35,7 @@ struct W4Weights {
 //         hold q * 2^-133, bits 4..7 q * 2^-129, both exactly.  One packed fused multiply-add by 2^127 normalises them
 //         and subtracts the zero point: (q - z) / 64 for the low nibble, (q - z) / 4 for the high one, exact.  The low
 //         nibbles are rows r, the high ones rows r + 8: the factor is a constant of the row and is put back on the fp32
-//         sums (kW4RowFactor).  Two rows' pairs cost two ANDs and half a shift this way, where placing all four nibbles
+//         sums (kFactorLow, kFactorHigh).  Two rows' pairs cost two ANDs and half a shift this way, where placing all four nibbles
 //         at the same position takes three shifts.
 //   fp16  The nibble is or-ed under the exponent of 1024: 1024 + q (low) or 1024 + 16 q (high); one packed fused
 //         multiply-add turns that into q - z, exact.

@@ -8,6 +8,7 @@ namespace mlk {
 int launch_w4_dense(const W4DenseParams& p, cudaStream_t s) {
     if (p.m <= 0 || p.m % 16 != 0) return fail(kInvalidArg, "gemm_layoutA_w4: m must be a positive multiple of 16 (got %d)", p.m);
     if (p.k <= 0) return fail(kInvalidArg, "gemm_layoutA_w4: k must be positive");
+    if (p.m > kW4MaxDim || p.k > kW4MaxDim) return fail(kUnsupported, "gemm_layoutA_w4: more than 2^28 rows or k");
     if (p.n < 0) return fail(kInvalidArg, "gemm_layoutA_w4: n must not be negative");
     if (p.w.group != 32 && p.w.group != 64 && p.w.group != 128)
         return fail(kInvalidArg, "gemm_layoutA_w4: groups of 32, 64 or 128 (got %d)", p.w.group);

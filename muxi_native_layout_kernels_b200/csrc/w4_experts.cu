@@ -2,8 +2,9 @@
 //
 // Sequence: alignment (routed slots grouped by expert, one work item per expert and up to 8, 32, 64 or 128 slots) -> with
 // more than a few slots per expert the token rows in slot order -> gate/up product with SiLU on the fp32 sums -> down
-// product, weighted, into one fp32 row per slot -> sum of a token's rows in slot order with one rounding.  The activation between the two products is rounded to the 16-bit activation type, as in
-// the 16-bit and e4m3 expert kernels.
+// product, weighted, into one fp32 row per slot -> sum of a token's rows in slot order with one rounding.  A single token takes two
+// launches instead: its slots are the work items, and clusters of them sum the result.  The activation between the two
+// products is rounded to the 16-bit activation type, as in the 16-bit and e4m3 expert kernels.
 #include <algorithm>
 #include <cmath>
 
@@ -87,6 +88,7 @@ long long w4_experts_workspace_bytes(int T, int E, int topk, int H, int I) {
 int launch_w4_experts(const W4ExpertsParams& p, cudaStream_t s) {
     if (p.T < 0 || p.E <= 0 || p.topk <= 0 || p.H <= 0 || p.I <= 0) return fail(kInvalidArg, "fused_experts_compute_w4: bad sizes");
     if (p.dtype != kBF16 && p.dtype != kFP16) return fail(kInvalidArg, "fused_experts_compute_w4: activations must be bf16 or fp16");
+    if (p.H > kW4MaxDim || p.I > kW4MaxDim / 2) return fail(kUnsupported, "fused_experts_compute_w4: more than 2^28 rows or k");
     if (p.H % 32 != 0 || p.I % 32 != 0)
         return fail(kInvalidArg, "fused_experts_compute_w4: hidden and intermediate sizes must be multiples of 32 (got %d, %d)", p.H, p.I);
     if (int st = check_weights(p.w1, p.H, "w1")) return st;
@@ -95,6 +97,8 @@ int launch_w4_experts(const W4ExpertsParams& p, cudaStream_t s) {
     if (!p.x || !p.topk_ids || !p.topk_weights || !p.y || !p.workspace) return fail(kInvalidArg, "fused_experts_compute_w4: null pointer");
     if (((uintptr_t)p.x | (uintptr_t)p.y | (uintptr_t)p.workspace) & 15)
         return fail(kInvalidArg, "fused_experts_compute_w4: activations, result and workspace must be 16-byte aligned");
+    if ((((uintptr_t)p.topk_ids | (uintptr_t)p.experts_map) & 3) || ((uintptr_t)p.topk_weights & 1))
+        return fail(kInvalidArg, "fused_experts_compute_w4: topk_ids, topk_weights or experts_map is not aligned");
     if (p.experts_map != nullptr && p.experts_map_len <= 0) return fail(kInvalidArg, "fused_experts_compute_w4: experts_map needs its length");
     const long long slots = (long long)p.T * p.topk;
     if (slots > (1 << 24)) return fail(kUnsupported, "fused_experts_compute_w4: more than 2^24 routed slots");

@@ -37,8 +37,8 @@ __device__ __forceinline__ void store16(void* base, size_t i, float v) {
     else reinterpret_cast<__nv_bfloat16*>(base)[i] = __float2bfloat16_rn(v);
 }
 
-// items: work items (exact for the dense products, an upper bound for the experts, whose number the device knows);
-// likely_items: what the grid is sized for.
+// MODE of both forms: 0 = dense product, 1 = the experts' gate/up product with SiLU, 2 = their down product.
+// items: work items (exact for the dense products, an upper bound for the experts, whose number the device knows).
 // tcgen05 form: np = tokens per tile (32, 64, 128; 256 in mode 0), sk = CTAs of a cluster along k, run = consecutive
 // row tiles of a CTA, matrices = experts (1 in mode 0), x_rows = rows of X.
 int launch_w4_umma(int mode, int wt, const W4KernelParams& p, const W4Weights& w, long long matrices, int x_rows, int np, int sk,
@@ -48,7 +48,8 @@ struct W4UmmaPlan {
     double us;                  // estimated time
 };
 W4UmmaPlan w4_umma_plan(int rows16, int n, int k);
-// With p.ids the experts' modes take a single token's slots (at most 8) as their items.
+// Streaming form: nt = 8-token column tiles, likely_items = what the split over k is chosen for.  With p.ids the experts'
+// modes take a single token's slots (at most 8) as their items.
 int launch_w4_mma(int mode, int wt, W4KernelParams p, const W4Weights& w, int items, int likely_items, int nt, cudaStream_t s);
 
 }  // namespace mlk

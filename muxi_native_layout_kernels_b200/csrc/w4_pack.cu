@@ -92,6 +92,7 @@ int launch_w4_groups(const void* src, void* dst, long long m, int groups, int el
     if (m < 0 || m % 16 != 0) return fail(kInvalidArg, "layoutA_w4_groups: m must be a multiple of 16 (got %lld)", m);
     if (groups <= 0) return fail(kInvalidArg, "layoutA_w4_groups: there must be at least one group");
     if (m > 0 && (!src || !dst)) return fail(kInvalidArg, "layoutA_w4_groups: null pointer");
+    if (elem == 2 && (((uintptr_t)src | (uintptr_t)dst) & 1)) return fail(kInvalidArg, "layoutA_w4_groups: pointers are not aligned");
     const long long n = m * groups;
     if (elem == 1)
         return launch_grid_stride("layoutA_w4_groups", w4_groups_kernel<uint8_t>, n, s, reinterpret_cast<const uint8_t*>(src),

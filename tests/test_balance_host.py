@@ -70,3 +70,19 @@ def test_c_entry_refuses_bad_arguments():
     assert lib.mlk_expert_counts(ok, None, -1, 2, 8, ok, None) == 1
     assert lib.mlk_router_balance_grad(ok, None, None, 4, 8, 1, 0, 0, None, None, ok, None) == 1
     assert lib.mlk_router_balance_grad(ok, None, None, 4, 8, 2, 0, 0, ok, None, ok, None) == 1
+
+
+def test_c_entry_refuses_sizes_and_addresses_out_of_range():
+    """More picks than a 32-bit count holds, and addresses that the types' alignment rules out."""
+    from muxi_native_layout_kernels_b200._lib import lib
+    ok = 1 << 20
+
+    def loss(logits=ok, ids=ok, cu=None, grad=None, T=50000, topk=2, dtype=0):
+        return lib.mlk_router_balance_loss(logits, ids, None, cu, T, 8, topk, 1, 0, 1.0, dtype, ok, ok, ok, grad, ok, 1 << 40, None)
+
+    assert loss(T=1 << 28, topk=8) == 2
+    assert loss(logits=ok + 1) == 1 and loss(logits=ok + 2, dtype=3) == 1
+    assert loss(ids=ok + 2) == 1 and loss(cu=ok + 2) == 1 and loss(grad=ok + 1) == 1
+    assert lib.mlk_router_balance_grad(ok + 1, None, None, 4, 8, 1, 0, 0, ok, None, ok, None) == 1
+    assert lib.mlk_expert_counts(ok, None, 1 << 28, 8, 8, ok, None) == 2
+    assert lib.mlk_expert_counts(ok + 1, None, 4, 2, 8, ok, None) == 1

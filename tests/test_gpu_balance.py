@@ -142,6 +142,32 @@ def test_autograd_and_upstream_gradient(dtype):
         assert torch.equal(mlk().router_balance_loss(leaf, ids.cuda(), 1, 0.5, **kw)[0], direct[0])
 
 
+@pytest.mark.parametrize("T", [40, 6000])
+def test_backward_pass_in_a_graph(T):
+    """Forward and backward captured together, no eager graph of the leaf alive, replayed with other logits."""
+    require_gpu()
+    (x, ids, _, _), other = inputs(T, 32, 4, "fp32", 5), inputs(T, 32, 4, "fp32", 6)[0]
+    leaf, ids = x.cuda().requires_grad_(), ids.cuda()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        mlk().router_balance_loss(leaf, ids)[0].backward()
+    torch.cuda.current_stream().wait_stream(side)
+    leaf.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, counts = mlk().router_balance_loss(leaf, ids)
+        loss.backward()
+    with torch.no_grad():
+        leaf.copy_(other)
+    for _ in range(2):
+        graph.replay()
+    want = mlk().router_balance_loss(leaf.detach(), ids, return_grad=True)
+    assert torch.equal(loss.detach(), want[0]) and torch.equal(counts, want[1])
+    # both forms sum in fp32 in orders of their own
+    assert (leaf.grad - want[2]).abs().max() <= want[2].abs().max() * 2.0 ** -15
+
+
 def test_unaligned_logits():
     require_gpu()
     x, ids, _, _ = inputs(31, 16, 2, "bf16", 6)

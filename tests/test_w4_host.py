@@ -82,3 +82,23 @@ def test_c_entries_refuse_bad_arguments():
         assert lib.mlk_layoutA_w4(*bad, None) == 1, bad
     for bad in ((ok, ok, 8, 2, 2), (ok, ok, 16, 0, 2), (ok, ok, 16, 2, 4), (ok, None, 16, 2, 2)):
         assert lib.mlk_layoutA_w4_groups(*bad, None) == 1, bad
+
+
+def test_c_entries_refuse_sizes_and_addresses_out_of_range():
+    """Sizes beyond the kernels' 32-bit row arithmetic and addresses that the types' alignment rules out."""
+    from muxi_native_layout_kernels_b200._lib import lib
+    ok, odd, big = 1 << 20, (1 << 20) + 1, (1 << 28) + 128
+
+    def gemm(m=32, k=64):
+        return lib.mlk_gemm_layoutA_w4(ok, ok, None, 32, ok, ok, m, 1, k, 0, 1.0, None, None, None)
+
+    assert gemm(m=big) == 2 and gemm(k=big) == 2 and gemm(m=2 ** 31 - 16) == 2
+
+    def experts(H=64, I=32, ids=ok, p=ok, mp=None):
+        return lib.mlk_fused_experts_compute_w4(ok, ok, None, 32, ok, ok, None, 32, ok, 4, 2, 2, H, I, ids, p, ok, 0, 0, mp, 2, ok,
+                                                1 << 62, None, None)
+
+    assert experts(H=big) == 2 and experts(I=big // 2) == 2 and experts(I=1 << 30) == 2
+    assert experts(ids=ok + 2) == 1 and experts(p=odd) == 1 and experts(mp=ok + 2) == 1
+    assert lib.mlk_layoutA_w4_groups(odd, ok, 16, 2, 2, None) == 1
+    assert lib.mlk_layoutA_w4_groups(ok, odd, 16, 2, 2, None) == 1
