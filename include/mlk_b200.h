@@ -340,21 +340,25 @@ int mlk_fused_experts_compute_static(const void* w1, const void* w2, const void*
  * groups, m a multiple of 16.  Laid out once at load time:
  *   q  row-major nibbles [m, k/2] (low nibble = even k) -> [m/16][ceil(k/64)][32][16 bytes]   mlk_layoutA_w4
  *   s, z  [m, k/group] -> [m/16][k/group][8][2], entry (r, h) = row r + 8 h of 16               mlk_layoutA_w4_groups
- * Lane l = 4 r + t of a block holds four little-endian 32-bit words; word j has the nibble pair p (bits 4p and 16 + 4p) of row r + 8 (p & 1), k = 64 block + 16 j + 4 t + 2 (p >> 1) and the next k.
+ * Lane l = 4 r + t of a block holds four little-endian 32-bit words; word j has the nibble pair p (bits 4p and 16 + 4p) of row
+ * r + 8 (p & 1), k = 64 block + 16 j + 4 t + 2 (p >> 1) and the next k.
  * Matrices stored back to back (the experts of a layer) are one matrix with all their rows. */
 
 /* inverse = 0: row-major src -> packed dst; inverse = 1: packed src -> row-major dst.  k % 32 == 0. */
 int mlk_layoutA_w4(const void* src, void* dst, int64_t m, int k, int inverse, mlk_stream_t s);
 /* elem_bytes: 2 (scales) or 1 (zero points). */
 int mlk_layoutA_w4_groups(const void* src, void* dst, int64_t m, int groups, int elem_bytes, mlk_stream_t s);
-/* C[n,m] = alpha * B[n,k] * W^T (+ bias), any n >= 0; dtype 0 / 1 = bf16 / fp16 scales, B, C and bias.  zeros may be NULL (8
- * everywhere); of each zero point the low four bits count.  status: sticky error word of the bounded waits, or NULL. */
+/* C[n,m] = alpha * B[n,k] * W^T (+ bias), any n >= 0, m and k up to 2^28; dtype 0 / 1 = bf16 / fp16 scales, B, C and bias.
+ * zeros may be NULL (8 everywhere); of each zero point the low four bits count.  Sums in fp32, rounded once.  Up to 16 tokens
+ * the weights' value is exact; larger calls multiply the value rounded to the activation type.  status: sticky error word
+ * of the bounded waits, or NULL. */
 int mlk_gemm_layoutA_w4(const void* A, const void* scales, const void* zeros, int group, const void* B, void* C, int m, int n,
                         int k, int dtype, float alpha, const void* bias, int32_t* status, mlk_stream_t s);
 /* Expert compute with 4-bit weights: y[t] = sum_j topk_weights[t,j] * W2_e (silu(Wgate_e x_t) * (Wup_e x_t)), e =
  * topk_ids[t,j] (through experts_map if given; ids without an expert here are skipped).  w1 [expert_count, 2 inter, hidden]
  * (gate rows, then up rows) and w2 [expert_count, hidden, inter] packed, with their own group sizes; hidden and inter
- * multiples of 32 and whole groups.  y [T, hidden] in the activation type, or fp32 un-rounded sums with out_fp32 != 0;
+ * multiples of 32 and whole groups.  Up to 4 routed slots per expert on average the weights' value is exact, above that it
+ * is rounded to the activation type, as the activation between the two products always is.  y [T, hidden] in the activation type, or fp32 un-rounded sums with out_fp32 != 0;
  * every element of y is written.  workspace: mlk_experts_w4_workspace_bytes(...) bytes, 16-byte aligned, contents
  * irrelevant, not shared by calls that can overlap on the GPU. */
 int64_t mlk_experts_w4_workspace_bytes(int batch_size, int expert_count, int topK, int hidden, int inter);
@@ -375,8 +379,8 @@ int mlk_fused_experts_compute_w4(const void* w1, const void* w1_scales, const vo
  * logits [tokens, num_experts], dtype 0 / 1 / 3 = bf16 / fp16 / fp32, num_experts <= 1024.  topk_ids int32 [tokens, topK], ids
  * outside [0, num_experts) count nowhere.  token_mask: bytes [tokens], 0 = not counted (NULL = all).  cu_seqlens: int32
  * [sequences + 1], not decreasing, tokens outside [cu[0], cu[sequences]) belong to no sequence; NULL = one sequence of all
- * tokens.  Logits of tokens that are not counted are not read and get the gradient 0; a token whose logits are all -inf
- * has p = 0.  dprob: fp32 [sequences, num_experts], receives d loss / d p (what mlk_router_balance_grad reads).  grad:
+ * tokens.  What the logits of tokens that are not counted hold has no influence, and their gradient is 0; a token whose
+ * logits are all -inf has p = 0.  tokens * topK < 2^31.  dprob: fp32 [sequences, num_experts], receives d loss / d p (what mlk_router_balance_grad reads).  grad:
  * NULL, or [tokens, num_experts] in the logits' type, receives d loss / d logits.  Sums in fp32 in a fixed order.
  * workspace: mlk_router_balance_workspace_bytes(...) bytes on the current device, contents irrelevant.  Where that is 0 (a
  * small batch, one kernel for the whole call) workspace may be NULL, and so may dprob. */

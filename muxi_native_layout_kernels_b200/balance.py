@@ -110,9 +110,11 @@ def router_balance_loss(gating_output: torch.Tensor, experts_ids: torch.Tensor, 
     ``gating_output [T, E]`` bf16, fp16 or fp32 logits (E <= 1024); ``experts_ids`` int32 ``[T, topk]``, ids outside
     ``[0, E)`` count nowhere.  ``token_mask [T]`` (bool or uint8): only tokens with a nonzero entry are counted.
     ``cu_seqlens`` int32 ``[B + 1]``, not decreasing: the loss is the mean over the B sequences (an empty one adds 0); tokens
-    behind the last sequence are in none.  Tokens that are not counted are not read and get the gradient 0; a token whose
-    logits are all -inf has no distribution and adds 0.  ``return_grad=True``: ``(loss, counts, d loss / d gating_output)``
-    in one call, for callers that write their backward pass by hand (nothing is recorded for autograd).
+    behind the last sequence are in none.  What the logits of tokens that are not counted hold (NaN included) has no
+    influence, and their gradient is 0; a token whose logits are all -inf has no distribution and adds 0.
+    ``return_grad=True``: ``(loss, counts, d loss / d gating_output)`` in one call, for callers that write their backward
+    pass by hand and for captured steps (nothing is recorded for autograd).  A recorded call can be captured together with its
+    backward pass as long as no graph recorded outside the capture still holds the same leaves.
     Probabilities, sums and the loss are fp32, added in a fixed order; the gradient is rounded once to the logits' type."""
     _checked(gating_output, experts_ids, score_fun, token_mask, cu_seqlens)
     if return_grad:

@@ -2,12 +2,17 @@
 //
 //   C[n, m] = alpha * sum_k W[m, k] x[n, k] (+ bias),   W = (q - z) s per group of 32, 64 or 128 k
 //
-// What bounds it: the packed weights, read once.  At 6.5 TB/s that is 46 weights per SM and cycle, so the work per weight
-// has to stay small: a word of eight weights becomes the 16-row operand of one m16n8k16 step with two ANDs, half a shift
-// and one packed FMA per two weights (w4.cuh), the zero point subtracted exactly on the way, and the scale multiplies the
-// fp32 sums of a group, not the weights.  Measured on the arithmetic alone (operands from shared memory, no other
-// traffic): 16.8 T weights/s with one column tile of 8 tokens, 11 T with two; HBM delivers 13 T.  More than 16 tokens go
-// to the tcgen05 kernel.
+// What bounds it: the packed weights, read once, and the instructions on them.  At 6.5 TB/s that is 46 weights per SM and
+// cycle, so the work per weight has to stay small: a word of eight weights becomes the 16-row operand of one m16n8k16 step
+// with four ANDs, a shift and four packed FMAs (w4.cuh), the zero point subtracted exactly on the way, and the scale
+// multiplies the fp32 sums of a group, not the weights.  Measured on the arithmetic alone (operands from shared memory, no
+// other traffic): 16.8 T weights/s with one column tile of 8 tokens, 11 T with two; HBM delivers 13 T; a copy of the
+// weights into shared memory alone takes 21 us for the 117 MB of 28672 x 8192, with the arithmetic 25.
+// Measured (us, and of the time that the bytes take at the copy bandwidth): 4096 x 4096 at 1 token 5.6 (1.3: one wave of
+// CTAs, latency), 28672 x 8192 at 8 tokens 31 (18.6), 4096 x 14336 fp16 with zero points at 16 tokens 17 (5.0), 8 of 128 experts of 2048 x 768 for one token 14.4 (3.0: two kernels of latency), 33
+// tokens on them 63 (42), 5 tokens on 8 experts of 4096 x 14336 118 (85).  At 28672 x 8192 and 8 tokens a word takes 16
+// warp instructions in all, and the issue slots are 54 % busy, the ALU pipe 45 %, the tensor pipe 27 %: the warps wait for
+// one another's pipes, not for memory.  More than 16 tokens go to the tcgen05 kernel.
 //
 // A warp owns RT tiles of 16 rows and every WK-th unit of 128 k; WR x WK = 8 warps share the rows and the k range of a CTA.
 // The CTA's activations and scales are staged in shared memory once, so that a unit costs one 8-byte shared load per step
@@ -15,10 +20,11 @@
 // 16-byte cp.async: a lane copies exactly the bytes that it will read itself, so the ring needs no barrier and costs no
 // registers.  The warps' partial sums meet in shared memory, the k parts of a cluster in distributed shared memory, both
 // in a fixed order: results do not depend on timing.
-// Measured and not used: activations and scales fetched by each warp from global memory (21 instead of 14 instructions per
-// word; 28672 x 8192 at 8 tokens 37 instead of 31 us); a persistent grid with an equal run of tiles per SM (31 us there, but
-// 80 instead of 64 us for 33 tokens on 128 small experts); activations kept in registers with the rows streaming past
-// (33 and 85 us: every few tiles all warps have to meet).
+// Measured and not used: activations and scales fetched by each warp from global memory (28672 x 8192 at 8 tokens 37
+// instead of 31 us); a persistent grid with an equal run of tiles per SM (31 us there, but 80 instead of 64 us for 33
+// tokens on 128 small experts); activations kept in registers with the rows streaming past (33 and 85 us: every few tiles
+// all warps have to meet); rings one unit deep (37 and 70 us); two row tiles per warp with rings of two / three units (31 / 34 us
+// there, 19 / 25 instead of 17.7 us at 16 tokens of 4096 x 14336, 61 / 62 us for 33 tokens on the experts).
 #include <algorithm>
 #include <array>
 #include <cmath>
