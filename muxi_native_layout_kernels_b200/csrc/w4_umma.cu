@@ -9,14 +9,18 @@
 //                        take the stages in turn, or, where a CTA holds a gate and an up tile, one tile each
 //   MMA (one thread)     tcgen05.mma with the weights in tensor memory and the token tile in shared memory
 // The decoded weight is (q - z) s rounded once to the activation type, the value a dequantised checkpoint holds: scaling
-// the fp32 sums instead would take one accumulator pass per group.  In bf16 the decode leaves a constant factor of the row (w4.cuh)
-// that is put back on the accumulator.
+// the fp32 sums instead would take one accumulator pass per group.  In bf16 the decode leaves a constant factor of the row
+// (w4.cuh) that is put back on the accumulator.
 // What bounds it: up to about 64 tokens the decode (13 packed instructions per word of eight weights) and the hand-offs
 // between the roles, at NP = 256 the tensor pipe.  Small grids split k over a cluster; partial tiles are added through
 // distributed shared memory in a fixed order.
 // Measured (us, and the floor by bytes or by the tensor peak): 14336 x 4096 with zero points per 32 at 61 tokens 17.2 (5.7;
 // issue slots 49 % busy, tensor pipe 27 %), 8192 x 8192 at 500 tokens 54 at full clocks, 62 under the power cap (40.6; tensor pipe
-// 62 %), 512 tokens x 8 on 128 experts of 2048 x 768 in fp16 with zero points 153, under the power cap 172 (51).
+// 62 %), 512 tokens x 8 on 128 experts of 2048 x 768 in fp16 with zero points 153, under the power cap 168 (51).
+// The parts of a stage overlap only in part: at 37888 x 8192 and 64 tokens (45 us) a copy without the stores to tensor memory
+// took 41, without the MMAs 36, without the decode 38, with none of them 30.  An MMA with its rows in tensor memory takes
+// 20 / 32 / 64 / 128 cycles at 32 / 64 / 128 / 256 tokens.  Three slots, six raw stages, or one CTA per SM with all of the
+// tensor memory (142 -> 167 us for 512 tokens on the experts in bf16) were no better.
 // A store to tensor memory in the 16 x 256-bit shape moves 254 bytes per SM and cycle (16 x 128 bit 455, 32 x 32 bit 372):
 // that shape is taken because it needs no exchange between lanes, and the stores are not what a stage waits for.
 #include <algorithm>
