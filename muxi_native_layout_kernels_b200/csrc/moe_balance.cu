@@ -145,13 +145,19 @@ __device__ __forceinline__ void scores(const Params& p, float (&x)[N], float (&o
 #pragma unroll
         for (int i = 0; i < N; ++i) s += x[i] = expf(x[i] - m);
     } else {
+        // sigmoid(x) = e^min(x,0) / (1 + e^-|x|), taken here over e^m, m the row's largest min(x,0): the factor cancels in p, no
+        // term overflows and the sum is at least 1/2, where the sigmoids themselves end below about -88 - ln E.  With a
+        // logit of 0 or more in the row m is 0.
+        float m = fminf(x[0], 0.f);
+#pragma unroll
+        for (int i = 1; i < N; ++i) m = fmaxf(m, fminf(x[i], 0.f));
+        m = group_max(m, p.lpr);
+        if (m == -INFINITY) m = 0.f;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            // both forms from exp(-|x|), which cannot overflow
             const float e = expf(-fabsf(x[i])), d = 1.f / (1.f + e);
-            const float pos = d, neg = e * d;
-            if constexpr (GRAD) one_minus[i] = x[i] >= 0.f ? neg : pos;
-            s += x[i] = x[i] != x[i] ? x[i] : (x[i] >= 0.f ? pos : neg);
+            if constexpr (GRAD) one_minus[i] = x[i] >= 0.f ? e * d : d;
+            s += x[i] = expf(fminf(x[i], 0.f) - m) * d;          // NaN stays NaN through d
         }
     }
     s = group_sum(s, p.lpr);

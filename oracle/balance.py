@@ -9,8 +9,7 @@ def probs(logits, score_fun):
     if score_fun == 0:
         p = torch.softmax(x, -1)
     else:
-        s = torch.sigmoid(x)
-        p = s / s.sum(-1, keepdim=True)
+        p = torch.softmax(torch.nn.functional.logsigmoid(x), -1)     # the sigmoids themselves end near -745
     return torch.where((x == -float("inf")).all(-1, keepdim=True), torch.zeros_like(p), p)
 
 
