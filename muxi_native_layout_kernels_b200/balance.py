@@ -14,6 +14,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+import torch.autograd.forward_ad as _forward
 
 from ._lib import lib
 from .ext import _chk, _cuda_contig, _ptr
@@ -114,9 +115,12 @@ def router_balance_loss(gating_output: torch.Tensor, experts_ids: torch.Tensor, 
     influence, and their gradient is 0; a token whose logits are all -inf has no distribution and adds 0.
     ``return_grad=True``: ``(loss, counts, d loss / d gating_output)`` in one call, for callers that write their backward
     pass by hand and for captured steps (nothing is recorded for autograd).  A recorded call can be captured together with its
-    backward pass as long as no graph recorded outside the capture still holds the same leaves.
+    backward pass as long as no graph recorded outside the capture still holds the same leaves.  Forward-mode derivatives (dual
+    tensors) are refused.
     Probabilities, sums and the loss are fp32, added in a fixed order; the gradient is rounded once to the logits' type."""
     _checked(gating_output, experts_ids, score_fun, token_mask, cu_seqlens)
+    if _forward._current_level >= 0:          # a dual tensor has no requires_grad: its tangent would be lost unseen
+        _chk(_forward.unpack_dual(gating_output).tangent is None, "router_balance_loss has no forward-mode derivative")
     if return_grad:
         loss, counts, _, grad = _loss(gating_output.detach(), experts_ids, score_fun, float(coef), token_mask, cu_seqlens, True)
         return loss, counts, grad

@@ -73,6 +73,22 @@ def test_sigmoid_rows_without_a_distribution_or_with_nan(T):
     assert torch.isnan(got[0]) and torch.isnan(got[2][8]).any() and torch.isfinite(got[2][9]).all()
 
 
+def test_forward_mode_is_refused():
+    """A dual tensor has no requires_grad; its tangent must not be dropped in silence."""
+    require_gpu()
+    import torch.autograd.forward_ad as fw
+    x, ids = torch.randn(6, 8, device="cuda"), torch.zeros(6, 2, dtype=torch.int32, device="cuda")
+    with fw.dual_level():
+        dual = fw.make_dual(x, torch.ones_like(x))
+        for kw in ({}, {"return_grad": True}):
+            with pytest.raises(RuntimeError, match="forward"):
+                mlk().router_balance_loss(dual, ids, **kw)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward"):
+            mlk().router_balance_loss(dual, ids)
+        mlk().router_balance_loss(x, ids)
+    mlk().router_balance_loss(x, ids)
+
+
 def test_oracle_used_here_holds_far_from_zero():
     """The 64-bit form at -1e4 against the closed form of two experts: p = 1 / (1 + e^d)."""
     x = torch.tensor([[-10000.0, -10001.0]], dtype=torch.float64)
