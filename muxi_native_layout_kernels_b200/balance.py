@@ -79,6 +79,24 @@ def _loss(x, ids, score_fun, coef, mask, cu, want_grad: bool):
     return loss, counts, ws, grad
 
 
+def _grad(grad_loss, x, dprob, mask, cu, score_fun):
+    grad = torch.empty_like(x)
+    _launch(x.get_device(), lib.mlk_router_balance_grad, x.data_ptr(), _ptr(mask), _ptr(cu), x.shape[0], x.shape[1],
+            1 if cu is None else cu.shape[0] - 1, score_fun, _CODES[x.dtype], dprob.data_ptr(), grad_loss.data_ptr(),
+            grad.data_ptr())
+    return grad
+
+
+class _BalanceGrad(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, grad_loss, x, dprob, mask, cu, score_fun):
+        return _grad(grad_loss, x, dprob, mask, cu, score_fun)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError("router_balance_loss can be differentiated once")
+
+
 class _BalanceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, ids, score_fun, coef, mask, cu):
@@ -91,16 +109,11 @@ class _BalanceLoss(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_loss, _):
-        if torch.is_grad_enabled():
-            raise RuntimeError("router_balance_loss can be differentiated once")
         if grad_loss is None:
             return None, None, None, None, None, None
-        x, dprob, mask, cu = ctx.saved_tensors
-        grad = torch.empty_like(x)
-        _launch(x.get_device(), lib.mlk_router_balance_grad, x.data_ptr(), _ptr(mask), _ptr(cu), x.shape[0], x.shape[1],
-                1 if cu is None else cu.shape[0] - 1, ctx.score_fun, _CODES[x.dtype], dprob.data_ptr(), grad_loss.data_ptr(),
-                grad.data_ptr())
-        return grad, None, None, None, None, None
+        # with create_graph the step is recorded itself, as one that has no derivative
+        call = _BalanceGrad.apply if torch.is_grad_enabled() else _grad
+        return call(grad_loss, *ctx.saved_tensors, ctx.score_fun), None, None, None, None, None
 
 
 def router_balance_loss(gating_output: torch.Tensor, experts_ids: torch.Tensor, score_fun: int = 0, coef: float = 1.0, *,
@@ -116,7 +129,7 @@ def router_balance_loss(gating_output: torch.Tensor, experts_ids: torch.Tensor, 
     ``return_grad=True``: ``(loss, counts, d loss / d gating_output)`` in one call, for callers that write their backward
     pass by hand and for captured steps (nothing is recorded for autograd).  A recorded call can be captured together with its
     backward pass as long as no graph recorded outside the capture still holds the same leaves.  Forward-mode derivatives (dual
-    tensors) are refused.
+    tensors) and second derivatives are refused.
     Probabilities, sums and the loss are fp32, added in a fixed order; the gradient is rounded once to the logits' type."""
     _checked(gating_output, experts_ids, score_fun, token_mask, cu_seqlens)
     if _forward._current_level >= 0:          # a dual tensor has no requires_grad: its tangent would be lost unseen

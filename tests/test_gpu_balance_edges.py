@@ -89,6 +89,25 @@ def test_forward_mode_is_refused():
     mlk().router_balance_loss(x, ids)
 
 
+@pytest.mark.parametrize("T", [6, 17000])
+def test_second_order_of_the_rest(T):
+    """create_graph over a loss of which this one is a part: the first derivatives are the usual ones, the other part
+    can be differentiated again, and only differentiating this one again is an error."""
+    require_gpu()
+    g = torch.Generator().manual_seed(T)
+    x = torch.randn(T, 8, generator=g).cuda().requires_grad_()
+    w = torch.randn(5, generator=g).cuda().requires_grad_()
+    ids = torch.randint(0, 8, (T, 2), generator=g, dtype=torch.int32).cuda()
+    want = mlk().router_balance_loss(x.detach(), ids, 0, 0.5, return_grad=True)[2]
+    total = mlk().router_balance_loss(x, ids, 0, 0.5)[0] + (w ** 3).sum()
+    gx, gw = torch.autograd.grad(total, (x, w), create_graph=True)
+    assert (gx.detach() - want).abs().max() <= want.abs().max() * 2.0 ** -15
+    (gw ** 2).sum().backward(retain_graph=True)
+    assert torch.allclose(w.grad, 36 * w.detach() ** 3, rtol=1e-5) and x.grad is None
+    with pytest.raises(RuntimeError, match="once"):
+        gx.sum().backward()
+
+
 def test_oracle_used_here_holds_far_from_zero():
     """The 64-bit form at -1e4 against the closed form of two experts: p = 1 / (1 + e^d)."""
     x = torch.tensor([[-10000.0, -10001.0]], dtype=torch.float64)
