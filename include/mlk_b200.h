@@ -357,7 +357,7 @@ int mlk_gemm_layoutA_w4(const void* A, const void* scales, const void* zeros, in
 /* Expert compute with 4-bit weights: y[t] = sum_j topk_weights[t,j] * W2_e (silu(Wgate_e x_t) * (Wup_e x_t)), e =
  * topk_ids[t,j] (through experts_map if given; ids without an expert here are skipped).  w1 [expert_count, 2 inter, hidden]
  * (gate rows, then up rows) and w2 [expert_count, hidden, inter] packed, with their own group sizes; hidden and inter
- * multiples of 32 and whole groups.  Up to 4 routed slots per expert on average the weights' value is exact, above that it
+ * multiples of 32 and whole groups; at most 1024 experts and 8257408 slots (batch_size * topK).  Up to 4 routed slots per expert on average the weights' value is exact, above that it
  * is rounded to the activation type, as the activation between the two products always is.  y [T, hidden] in the activation type, or fp32 un-rounded sums with out_fp32 != 0;
  * every element of y is written.  workspace: mlk_experts_w4_workspace_bytes(...) bytes, 16-byte aligned, contents
  * irrelevant, not shared by calls that can overlap on the GPU. */

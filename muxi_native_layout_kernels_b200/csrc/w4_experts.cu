@@ -16,6 +16,11 @@ namespace mlk {
 
 namespace {
 
+// Experts: what the alignment takes.  Slots: the work items of a launch are its grid's z dimension, and from 80 slots an
+// expert on they hold 128 slots each, with one unfilled per expert at worst.
+constexpr int kMaxExperts = 1024;
+constexpr int kMaxSlots = (65535 - kMaxExperts) * 128;
+
 constexpr long long align256(long long b) { return (b + 255) / 256 * 256; }
 
 struct Layout {
@@ -101,7 +106,8 @@ int launch_w4_experts(const W4ExpertsParams& p, cudaStream_t s) {
         return fail(kInvalidArg, "fused_experts_compute_w4: topk_ids, topk_weights or experts_map is not aligned");
     if (p.experts_map != nullptr && p.experts_map_len <= 0) return fail(kInvalidArg, "fused_experts_compute_w4: experts_map needs its length");
     const long long slots = (long long)p.T * p.topk;
-    if (slots > (1 << 24)) return fail(kUnsupported, "fused_experts_compute_w4: more than 2^24 routed slots");
+    if (p.E > kMaxExperts) return fail(kUnsupported, "fused_experts_compute_w4: at most %d experts (got %d)", kMaxExperts, p.E);
+    if (slots > kMaxSlots) return fail(kUnsupported, "fused_experts_compute_w4: at most %d routed slots (got %lld)", kMaxSlots, slots);
     const Layout l = layout(p.T, p.E, p.topk, p.H, p.I);
     if (p.workspace_bytes < l.bytes)
         return fail(kInvalidArg, "fused_experts_compute_w4: workspace holds %lld bytes, needs %lld", p.workspace_bytes, l.bytes);

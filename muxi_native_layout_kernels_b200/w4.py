@@ -171,7 +171,7 @@ def fused_experts_compute_w4(w1, w1_scales, w2, w2_scales, activations, topk_ids
     int32 ``[T, topk]``, ``topk_weights`` in the activations' type.  ``experts_map``: global -> local expert or -1, as in
     ``fused_experts_compute``; ids without an expert here contribute nothing.  ``out_dtype=torch.float32`` gives the
     un-rounded sums; ``out`` receives the result (every element is written).  A token's experts are added in
-    slot order in fp32 with one rounding.  Up to 4 routed slots per expert on average the weights' value is exact; above
+    slot order in fp32 with one rounding.  At most 1024 experts and 8257408 slots (T * topk).  Up to 4 routed slots per expert on average the weights' value is exact; above
     that it is rounded to the activation type, as the activation between the two products always is."""
     x = activations
     _chk(x.is_cuda and x.is_contiguous(), "activations must be a contiguous CUDA tensor")
