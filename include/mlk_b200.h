@@ -382,7 +382,7 @@ int mlk_fused_experts_compute_w4(const void* w1, const void* w1_scales, const vo
  * tokens.  What the logits of tokens that are not counted hold has no influence, and their gradient is 0; a token whose
  * logits are all -inf has p = 0.  tokens * topK < 2^31.  dprob: fp32 [sequences, num_experts], receives d loss / d p (what mlk_router_balance_grad reads).  grad:
  * NULL, or [tokens, num_experts] in the logits' type, receives d loss / d logits.  Sums in fp32 in a fixed order.
- * workspace: mlk_router_balance_workspace_bytes(...) bytes on the current device, contents irrelevant.  Where that is 0 (a
+ * workspace: mlk_router_balance_workspace_bytes(...) bytes on the current device, 4-byte aligned, contents irrelevant.  Where that is 0 (a
  * small batch, one kernel for the whole call) workspace may be NULL, and so may dprob. */
 int64_t mlk_router_balance_workspace_bytes(int tokens, int num_experts, int sequences);
 int mlk_router_balance_loss(const void* logits, const int32_t* topk_ids, const void* token_mask, const int32_t* cu_seqlens,

@@ -621,6 +621,8 @@ int check(const BalanceParams& b, const char* who) {
     const uintptr_t elem = b.dtype == kF32 ? 3 : 1;
     if ((((uintptr_t)b.logits | (uintptr_t)b.grad) & elem) || (((uintptr_t)b.ids | (uintptr_t)b.cu_seqlens) & 3))
         return fail(kInvalidArg, "%s: logits, grad, topk_ids or cu_seqlens is not aligned", who);
+    if (((uintptr_t)b.loss | (uintptr_t)b.counts | (uintptr_t)b.u | (uintptr_t)b.grad_loss) & 3)
+        return fail(kInvalidArg, "%s: loss, counts, dprob or grad_loss is not aligned", who);
     return kOk;
 }
 
@@ -670,6 +672,7 @@ int launch_balance_loss(const BalanceParams& b, void* workspace, long long works
         return launch("router_balance_loss", kern, small, kSmallThreads, (rows * b.E + 3 * (size_t)b.B * b.E + b.B) * 4, s, p, small);
     }
     const long long records = (long long)q.runs + b.B;
+    if ((uintptr_t)workspace & 3) return fail(kInvalidArg, "router_balance_loss: workspace is not aligned");
     if (workspace_bytes < (records * b.E * 2 + records) * 4)
         return fail(kInvalidArg, "router_balance_loss: workspace holds %lld bytes, needs %lld", workspace_bytes, (records * b.E * 2 + records) * 4);
     p.P = reinterpret_cast<float*>(workspace);
@@ -704,7 +707,7 @@ int launch_expert_counts(const int32_t* ids, const uint8_t* mask, int T, int top
     if (E < 1 || E > kBalanceMaxExperts) return fail(kUnsupported, "expert_counts: 1 <= experts <= %d (got %d)", kBalanceMaxExperts, E);
     if ((long long)T * topk > 0x7FFFFFFF) return fail(kUnsupported, "expert_counts: counts of more than 2^31 - 1 picks");
     if (!counts || (T > 0 && !ids)) return fail(kInvalidArg, "expert_counts: null pointer");
-    if ((uintptr_t)ids & 3) return fail(kInvalidArg, "expert_counts: topk_ids is not aligned");
+    if (((uintptr_t)ids | (uintptr_t)counts) & 3) return fail(kInvalidArg, "expert_counts: topk_ids or counts is not aligned");
     cudaError_t e = cudaMemsetAsync(counts, 0, (size_t)E * 4, s);
     if (e != cudaSuccess) return fail(kCudaError, "expert_counts: %s", cudaGetErrorString(e));
     if (T == 0) return kOk;

@@ -17,7 +17,7 @@ int launch_w4_dense(const W4DenseParams& p, cudaStream_t s) {
     if (!p.w.q || !p.w.s || (p.n > 0 && (!p.X || !p.C))) return fail(kInvalidArg, "gemm_layoutA_w4: null pointer");
     if (((uintptr_t)p.w.q | (uintptr_t)p.w.s | (uintptr_t)p.w.z | (uintptr_t)p.X | (uintptr_t)p.C) & 15)
         return fail(kInvalidArg, "gemm_layoutA_w4: A, scales, zeros, B and C must be 16-byte aligned");
-    if ((uintptr_t)p.bias & 1) return fail(kInvalidArg, "gemm_layoutA_w4: bias is not aligned");
+    if (((uintptr_t)p.bias & 1) || ((uintptr_t)p.status & 3)) return fail(kInvalidArg, "gemm_layoutA_w4: bias or status is not aligned");
     if (p.n == 0) return kOk;
 
     W4KernelParams g{};

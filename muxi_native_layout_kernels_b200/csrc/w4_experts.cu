@@ -102,8 +102,8 @@ int launch_w4_experts(const W4ExpertsParams& p, cudaStream_t s) {
     if (!p.x || !p.topk_ids || !p.topk_weights || !p.y || !p.workspace) return fail(kInvalidArg, "fused_experts_compute_w4: null pointer");
     if (((uintptr_t)p.x | (uintptr_t)p.y | (uintptr_t)p.workspace) & 15)
         return fail(kInvalidArg, "fused_experts_compute_w4: activations, result and workspace must be 16-byte aligned");
-    if ((((uintptr_t)p.topk_ids | (uintptr_t)p.experts_map) & 3) || ((uintptr_t)p.topk_weights & 1))
-        return fail(kInvalidArg, "fused_experts_compute_w4: topk_ids, topk_weights or experts_map is not aligned");
+    if ((((uintptr_t)p.topk_ids | (uintptr_t)p.experts_map | (uintptr_t)p.status) & 3) || ((uintptr_t)p.topk_weights & 1))
+        return fail(kInvalidArg, "fused_experts_compute_w4: topk_ids, topk_weights, experts_map or status is not aligned");
     if (p.experts_map != nullptr && p.experts_map_len <= 0) return fail(kInvalidArg, "fused_experts_compute_w4: experts_map needs its length");
     const long long slots = (long long)p.T * p.topk;
     if (p.E > kMaxExperts) return fail(kUnsupported, "fused_experts_compute_w4: at most %d experts (got %d)", kMaxExperts, p.E);
