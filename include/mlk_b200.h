@@ -344,7 +344,7 @@ int mlk_fused_experts_compute_static(const void* w1, const void* w2, const void*
  * r + 8 (p & 1), k = 64 block + 16 j + 4 t + 2 (p >> 1) and the next k.
  * Matrices stored back to back (the experts of a layer) are one matrix with all their rows. */
 
-/* inverse = 0: row-major src -> packed dst; inverse = 1: packed src -> row-major dst.  k % 32 == 0. */
+/* inverse = 0: row-major src -> packed dst; inverse = 1: packed src -> row-major dst.  k % 32 == 0, k up to 2^28. */
 int mlk_layoutA_w4(const void* src, void* dst, int64_t m, int k, int inverse, mlk_stream_t s);
 /* elem_bytes: 2 (scales) or 1 (zero points). */
 int mlk_layoutA_w4_groups(const void* src, void* dst, int64_t m, int groups, int elem_bytes, mlk_stream_t s);

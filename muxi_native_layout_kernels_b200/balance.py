@@ -18,7 +18,7 @@ import torch.autograd.forward_ad as _forward
 
 from ._lib import lib
 from .ext import _chk, _cuda_contig, _ptr
-from .w4 import _launch, _same_device
+from .w4 import _LIMIT, _fits, _launch, _same_device
 
 __all__ = ["router_balance_loss", "expert_counts"]
 
@@ -38,11 +38,11 @@ def _checked(x, ids, score_fun, mask, cu):
     d, xs, s = x.get_device(), x.shape, ids.shape
     if (x.is_cuda and ids.get_device() == d and x.is_contiguous() and ids.is_contiguous() and x.dtype in _CODES
             and ids.dtype is torch.int32 and len(xs) == 2 and len(s) == 2 and xs[1] > 0 and s[0] == xs[0] and s[1] > 0
-            and score_fun in (0, 1)
+            and score_fun in (0, 1) and xs[0] < _LIMIT and xs[1] < _LIMIT and s[1] < _LIMIT
             and (mask is None or (mask.get_device() == d and mask.is_contiguous() and mask.shape == xs[:1]
                                   and (mask.dtype is torch.bool or mask.dtype is torch.uint8)))
             and (cu is None or (cu.get_device() == d and cu.is_contiguous() and cu.dtype is torch.int32 and cu.dim() == 1
-                                and cu.shape[0] >= 2))):
+                                and 2 <= cu.shape[0] <= _LIMIT))):
         return
     _cuda_contig(x, "gating_output")
     _cuda_contig(ids, "experts_ids")
@@ -56,6 +56,7 @@ def _checked(x, ids, score_fun, mask, cu):
         _cuda_contig(cu, "cu_seqlens")
         _chk(cu.dtype == torch.int32 and cu.dim() == 1 and cu.numel() >= 2, "cu_seqlens must be int32 [sequences + 1]")
     _same_device(x, (ids, "experts_ids"), (mask, "token_mask"), (cu, "cu_seqlens"))
+    _fits(T, x.size(1), ids.size(1), 0 if cu is None else cu.numel() - 1)
     raise RuntimeError("router_balance_loss: bad arguments")
 
 
@@ -150,6 +151,7 @@ def expert_counts(experts_ids: torch.Tensor, num_experts: int, token_mask: Optio
     T, topk = experts_ids.shape
     mask = _mask_ptr(token_mask, T)
     _same_device(experts_ids, (token_mask, "token_mask"))
+    _fits(T, topk, num_experts)
     counts = experts_ids.new_empty((num_experts,))
     _launch(experts_ids.get_device(), lib.mlk_expert_counts, experts_ids.data_ptr(), mask, T, topk, num_experts, counts.data_ptr())
     return counts

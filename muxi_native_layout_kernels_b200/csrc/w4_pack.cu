@@ -80,6 +80,7 @@ int launch_grid_stride(const char* what, void (*kern)(KArgs...), long long n, cu
 int launch_w4_pack(const void* src, void* dst, long long m, int k, int inverse, cudaStream_t s) {
     if (m < 0 || m % 16 != 0) return fail(kInvalidArg, "layoutA_w4: m must be a multiple of 16 (got %lld)", m);
     if (k <= 0 || k % 32 != 0) return fail(kInvalidArg, "layoutA_w4: k must be a positive multiple of 32 (got %d)", k);
+    if (k > kW4MaxDim) return fail(kUnsupported, "layoutA_w4: more than 2^28 k");
     if (m > 0 && (!src || !dst)) return fail(kInvalidArg, "layoutA_w4: null pointer");
     if (((uintptr_t)src | (uintptr_t)dst) & 15) return fail(kInvalidArg, "layoutA_w4: pointers must be 16-byte aligned");
     const int kc = (k + kW4BlockK - 1) / kW4BlockK;

@@ -27,6 +27,7 @@ __all__ = ["layoutA_w4", "layoutA_w4_inverse", "layoutA_w4_groups", "gemv_layout
            "fused_experts_compute_w4"]
 
 _GROUPS = (32, 64, 128)
+_LIMIT = 2 ** 31        # the C interface's sizes are 32-bit integers, and ctypes cuts off what is longer
 _CODES = {torch.bfloat16: 0, torch.float16: 1}
 _device_of_thread = torch._C._cuda_getDevice
 _stream_of = torch._C._cuda_getCurrentRawStream
@@ -55,14 +56,19 @@ def _same_device(like: torch.Tensor, *named) -> None:
             _chk(t.device == like.device, f"{name} must be on the same device as the activations")
 
 
+def _fits(*sizes) -> None:
+    _chk(max(sizes) < _LIMIT, "sizes of 2^31 and more are not supported")
+
+
 def layoutA_w4(W: torch.Tensor) -> torch.Tensor:
     """Row-major packed nibbles ``[m, k/2]`` uint8 (low nibble = even k) -> ``[m/16, ceil(k/64), 32, 16]``; a 3-D
-    ``[E, m, k/2]`` keeps its leading dimension.  m % 16 == 0, k % 32 == 0."""
+    ``[E, m, k/2]`` keeps its leading dimension.  m % 16 == 0, k % 32 == 0, k up to 2^28."""
     _cuda_contig(W, "W")
     _chk(W.dtype == torch.uint8, "W must be a uint8 tensor of packed nibbles")
     _chk(W.dim() in (2, 3), "W must be a 2D or 3D tensor")
     m, k = W.shape[-2], 2 * W.shape[-1]
     _chk(m % 16 == 0 and k % 32 == 0 and k > 0, "layoutA_w4 needs m % 16 == 0 and k % 32 == 0")
+    _fits(k)
     out = torch.empty(W.shape[:-2] + (m // 16, (k + 63) // 64, 32, 16), dtype=torch.uint8, device=W.device)
     rows = m * (W.shape[0] if W.dim() == 3 else 1)
     _launch(W.get_device(), lib.mlk_layoutA_w4, W.data_ptr(), out.data_ptr(), rows, k, 0)
@@ -74,6 +80,7 @@ def layoutA_w4_inverse(A: torch.Tensor, k: int) -> torch.Tensor:
     _cuda_contig(A, "A")
     R, kc = _packed_dims(A, "A")
     _chk(k > 0 and k % 32 == 0 and (k + 63) // 64 == kc, "k does not match the packed weights")
+    _fits(k)
     out = torch.empty(A.shape[:-4] + (R * 16, k // 2), dtype=torch.uint8, device=A.device)
     _launch(A.get_device(), lib.mlk_layoutA_w4, A.data_ptr(), out.data_ptr(), out.numel() // (k // 2), k, 1)
     return out
@@ -87,6 +94,7 @@ def layoutA_w4_groups(values: torch.Tensor) -> torch.Tensor:
     _chk(values.dim() in (2, 3), "values must be a 2D or 3D tensor")
     m, G = values.shape[-2:]
     _chk(m % 16 == 0 and G > 0, "layoutA_w4_groups needs m % 16 == 0 and at least one group")
+    _fits(G)
     out = torch.empty(values.shape[:-2] + (m // 16, G, 8, 2), dtype=values.dtype, device=values.device)
     rows = m * (values.shape[0] if values.dim() == 3 else 1)
     _launch(values.get_device(), lib.mlk_layoutA_w4_groups, values.data_ptr(), out.data_ptr(), rows, G, values.element_size())
@@ -146,6 +154,7 @@ def gemm_layoutA_w4(A, scales, B, alpha: float = 1, beta: float = 0, zeros=None,
     n, k = B.shape
     group = _group(A, scales, zeros, B, k, "A")
     m = A.shape[0] * 16
+    _fits(m, n, k)
     if bias is not None:
         _same_device(B, (bias, "bias"))
         bias = _bias_ptr(bias, B, m)
@@ -195,6 +204,8 @@ def fused_experts_compute_w4(w1, w1_scales, w2, w2_scales, activations, topk_ids
     if experts_map is not None:
         _same_device(x, (experts_map, "experts_map"))
         mp, ml = _map_args(experts_map)
+    topk = ids[1]
+    _fits(T, E, topk, H, I, ml)
     dtype = x.dtype if out_dtype is None else out_dtype
     _chk(dtype is x.dtype or dtype is torch.float32, "out_dtype must be the activation data type or torch.float32")
     if out is None:
@@ -202,7 +213,6 @@ def fused_experts_compute_w4(w1, w1_scales, w2, w2_scales, activations, topk_ids
     else:
         _chk(out.get_device() == d and out.is_contiguous() and out.shape == x.shape and out.dtype is dtype,
              "out must be a contiguous [T, H] in the result's data type on the activations' device")
-    topk = ids[1]
     nbytes = lib.mlk_experts_w4_workspace_bytes(T, E, topk, H, I)
     ws = x.new_empty((nbytes,), dtype=torch.uint8)
     _launch(d, lib.mlk_fused_experts_compute_w4, w1.data_ptr(), w1_scales.data_ptr(), _ptr(w1_zeros), g1, w2.data_ptr(),
