@@ -18,7 +18,7 @@ import torch.autograd.forward_ad as _forward
 
 from ._lib import lib
 from .ext import _chk, _cuda_contig, _ptr
-from .w4 import _LIMIT, _fits, _launch, _same_device
+from .w4 import _LIMIT, _device_of_thread, _fits, _launch, _same_device
 
 __all__ = ["router_balance_loss", "expert_counts"]
 
@@ -62,6 +62,9 @@ def _checked(x, ids, score_fun, mask, cu):
 
 def _loss(x, ids, score_fun, coef, mask, cu, want_grad: bool):
     """(loss, counts, d loss / d p behind the workspace's start, gradient or None), on the current stream."""
+    if _device_of_thread() != x.get_device():             # the size of the workspace is the current device's
+        with torch.cuda.device(x.get_device()):
+            return _loss(x, ids, score_fun, coef, mask, cu, want_grad)
     T, E = x.shape
     B = 1 if cu is None else cu.shape[0] - 1
     loss = x.new_empty((), dtype=torch.float32)
