@@ -154,7 +154,8 @@ def gemm_layoutA_w4(A, scales, B, alpha: float = 1, beta: float = 0, zeros=None,
     n, k = B.shape
     group = _group(A, scales, zeros, B, k, "A")
     m = A.shape[0] * 16
-    _fits(m, n, k)
+    if m >= _LIMIT or n >= _LIMIT or k >= _LIMIT:
+        _fits(m, n, k)
     if bias is not None:
         _same_device(B, (bias, "bias"))
         bias = _bias_ptr(bias, B, m)
@@ -205,7 +206,8 @@ def fused_experts_compute_w4(w1, w1_scales, w2, w2_scales, activations, topk_ids
         _same_device(x, (experts_map, "experts_map"))
         mp, ml = _map_args(experts_map)
     topk = ids[1]
-    _fits(T, E, topk, H, I, ml)
+    if T >= _LIMIT or E >= _LIMIT or topk >= _LIMIT or H >= _LIMIT or I >= _LIMIT or ml >= _LIMIT:
+        _fits(T, E, topk, H, I, ml)
     dtype = x.dtype if out_dtype is None else out_dtype
     _chk(dtype is x.dtype or dtype is torch.float32, "out_dtype must be the activation data type or torch.float32")
     if out is None:
