@@ -50,13 +50,14 @@ constexpr int conv_slots(int na, int np) {
     return na == 2 ? fit : fit / 2 * 2;
 }
 constexpr int raw_stages(int na) { return na == 2 ? 3 : 4; }
+// Dense products with small grids split k over a cluster: the partial tiles fit into the rings up to 128 tokens.
+constexpr bool can_split(int mode, int np) { return mode == 0 && np <= 128; }
 constexpr int token_stages(int np) { return np >= 256 ? 2 : (np >= 128 ? 2 : 3); }
 
 struct UmmaParams {
     W4KernelParams k;
     int stages;                 // stages of 128 k
     int run;                    // consecutive row tiles of a CTA (1 where a cluster splits k)
-    int sbytes;                 // bytes of a raw stage and weight tile: packed, scales, zero points
     int* status;
 };
 
@@ -116,7 +117,7 @@ __global__ void __launch_bounds__(kThreads, tmem_columns(MODE == 1 ? 2 : 1, NP) 
 
     const W4KernelParams& p = u.k;
     const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31;
-    const int row_tiles = (p.out_tiles + 7) / 8, tile = blockIdx.x * u.run, rank = blockIdx.y, SK = gridDim.y;
+    const int row_tiles = (p.out_tiles + 7) / 8, tile = blockIdx.x * u.run, rank = can_split(MODE, NP) ? blockIdx.y : 0, SK = can_split(MODE, NP) ? gridDim.y : 1;
     const int run = min(u.run, row_tiles - tile);
 
     const bool early = MODE == 0 && static_weights;  // weights may be fetched before the kernel in front has finished
@@ -128,7 +129,7 @@ __global__ void __launch_bounds__(kThreads, tmem_columns(MODE == 1 ? 2 : 1, NP) 
     } else {
         const int items = p.worklist[0].x;
         const int4 item = p.worklist[1 + blockIdx.z];
-        if ((int)blockIdx.z >= items) return;    // uniform over the cluster
+        if ((int)blockIdx.z >= items) return;
         mat = item.x; pos0 = item.y; ntok = item.z; row0 = item.w;
     }
     if constexpr (MODE == 2) {
@@ -406,71 +407,57 @@ __global__ void __launch_bounds__(kThreads, tmem_columns(MODE == 1 ? 2 : 1, NP) 
     __syncwarp();
 
     // ---- cluster: partial tiles over the k parts ----
-    if (SK > 1) {
-        const int rows_left = p.out_tiles * 16 - tile * kTileM;        // rows of the matrix in this tile
-        constexpr int kChunk = NP < 64 ? NP : 64;                      // tokens of one pass through shared memory
-        // [which][token][row] of a chunk of tokens in the (idle) rings, added over the cluster in rank order
-        float* const red = reinterpret_cast<float*>(base_ptr);
-        uint32_t remote[8];
+    if constexpr (can_split(MODE, NP)) {
+        if (SK > 1) {
+            const int rows_left = p.out_tiles * 16 - tile * kTileM;        // rows of the matrix in this tile
+            constexpr int kChunk = NP < 64 ? NP : 64;                      // tokens of one pass through shared memory
+            // [token][row] of a chunk of tokens in the (idle) rings, added over the cluster in rank order
+            float* const red = reinterpret_cast<float*>(base_ptr);
+            uint32_t remote[8];
 #pragma unroll
-        for (int q = 0; q < 8; ++q)
-            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote[q]) : "r"(base), "r"(q < SK ? q : 0));
+            for (int q = 0; q < 8; ++q)
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote[q]) : "r"(base), "r"(q < SK ? q : 0));
 #pragma unroll 1
-        for (int cb = 0; cb < NP; cb += kChunk) {
-            if (warp >= 2 && !abort_flag) {
-                const int quad = warp & 3, set = (warp - 2) >> 2, lrow = quad * 32 + lane;
-                const float f = (lrow & 8) ? D::kFactorHigh : D::kFactorLow;
-#pragma unroll
-                for (int w = 0; w < NA; ++w)
+            for (int cb = 0; cb < NP; cb += kChunk) {
+                if (warp >= 2 && !abort_flag) {
+                    const int quad = warp & 3, set = (warp - 2) >> 2, lrow = quad * 32 + lane;
+                    const float f = (lrow & 8) ? D::kFactorHigh : D::kFactorLow;
 #pragma unroll
                     for (int c0 = 0; c0 < kChunk / 2; c0 += 16) {
                         const int c = set * (kChunk / 2) + c0;
                         uint32_t a[16];
-                        tmem_ld16(tmem + ((uint32_t)(quad * 32) << 16) + w * NP + cb + c, a);
+                        tmem_ld16(tmem + ((uint32_t)(quad * 32) << 16) + cb + c, a);
                         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) red[(w * kChunk + c + i) * kTileM + lrow] = f * __uint_as_float(a[i]);
+                        for (int i = 0; i < 16; ++i) red[(c + i) * kTileM + lrow] = f * __uint_as_float(a[i]);
                     }
-            }
-            __syncwarp();
-            asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-            // this rank's share of the tokens, four rows of one token per thread and step
-            const int left = max(0, min(kChunk, ntok - cb));
-            for (int e = left * rank / SK * 32 + tid; e < left * (rank + 1) / SK * 32; e += kThreads) {
-                const int c = e >> 5, lrow = (e & 31) * 4, row = tile * kTileM + lrow;
-                float4 v[NA];
-#pragma unroll
-                for (int w = 0; w < NA; ++w) {
-                    v[w] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    const uint32_t off = 4u * ((w * kChunk + c) * kTileM + lrow);
+                }
+                __syncwarp();
+                asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+                // this rank's share of the tokens, four rows of one token per thread and step
+                const int left = max(0, min(kChunk, ntok - cb));
+                for (int e = left * rank / SK * 32 + tid; e < left * (rank + 1) / SK * 32; e += kThreads) {
+                    const int c = e >> 5, lrow = (e & 31) * 4, row = tile * kTileM + lrow;
+                    const uint32_t off = 4u * (c * kTileM + lrow);
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                     for (int q = 0; q < 8; ++q)
                         if (q < SK) {
                             float4 o;
                             asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
                                          : "=f"(o.x), "=f"(o.y), "=f"(o.z), "=f"(o.w) : "r"(remote[q] + off) : "memory");
-                            v[w].x += o.x; v[w].y += o.y; v[w].z += o.z; v[w].w += o.w;
+                            v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
                         }
-                }
-                if (lrow >= rows_left) continue;                       // whole 16-row groups are in or out
-                if constexpr (MODE == 0) {
+                    if (lrow >= rows_left) continue;                       // whole 16-row groups are in or out
                     float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
                     if (p.bias) b = make_float4(load_scalar16<WT>(p.bias, row), load_scalar16<WT>(p.bias, row + 1), load_scalar16<WT>(p.bias, row + 2), load_scalar16<WT>(p.bias, row + 3));
                     *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.C) + (size_t)(row0 + cb + c) * ld + row) =
-                        make_uint2(pack2<WT>(fmaf(p.alpha, v[0].x, b.x), fmaf(p.alpha, v[0].y, b.y)),
-                                   pack2<WT>(fmaf(p.alpha, v[0].z, b.z), fmaf(p.alpha, v[0].w, b.w)));
-                } else if constexpr (MODE == 1) {
-                    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.C) + (size_t)(row0 + cb + c) * ld + row) =
-                        make_uint2(pack2<WT>(silu_mul(v[0].x, v[NA - 1].x), silu_mul(v[0].y, v[NA - 1].y)),
-                                   pack2<WT>(silu_mul(v[0].z, v[NA - 1].z), silu_mul(v[0].w, v[NA - 1].w)));
-                } else {
-                    const float t = weight_of[cb + c];
-                    *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.C) + (size_t)slot_of[cb + c] * ld + row) =
-                        make_float4(t * v[0].x, t * v[0].y, t * v[0].z, t * v[0].w);
+                        make_uint2(pack2<WT>(fmaf(p.alpha, v.x, b.x), fmaf(p.alpha, v.y, b.y)),
+                                   pack2<WT>(fmaf(p.alpha, v.z, b.z), fmaf(p.alpha, v.w, b.w)));
                 }
+                __syncwarp();
+                asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
             }
-            __syncwarp();
-            asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
         }
     }
 
@@ -565,7 +552,7 @@ W4UmmaPlan w4_umma_plan(int rows16, int n, int k) {
     W4UmmaPlan best{32, 1, 1e30};
     for (int np = 32; np <= 256; np *= 2) {
         const int tokens = (n + np - 1) / np;
-        for (int sk = 1; sk <= (np == 256 ? 1 : 8) && sk <= stages; ++sk) {
+        for (int sk = 1; sk <= (can_split(0, np) ? 8 : 1) && sk <= stages; ++sk) {
             const double us = estimate(tiles, tokens, stages, np, sk);
             if (us < best.us) best = W4UmmaPlan{np, sk, us};
         }
@@ -590,7 +577,7 @@ int launch_w4_umma(int mode, int wt, const W4KernelParams& kp, const W4Weights& 
     if (kern == nullptr) return fail(kInvalidArg, "w4 (tcgen05): token tile %d is not built", np);
     if (sk < 1 || sk > 8 || sk > u.stages) return fail(kInvalidArg, "w4 (tcgen05): cluster size %d out of range", sk);
     if (sk > 1 && u.run > 1) return fail(kInvalidArg, "w4 (tcgen05): a cluster takes one row tile");
-    if (sk > 1 && np > 128) return fail(kInvalidArg, "w4 (tcgen05): k is not split with %d tokens per tile", np);
+    if (sk > 1 && !can_split(mode, np)) return fail(kInvalidArg, "w4 (tcgen05): k is not split in mode %d with %d tokens per tile", mode, np);
     if (encode_fn() == nullptr) return fail(kUnsupported, "w4 (tcgen05): cuTensorMapEncodeTiled is not available");
     if (items > 65535) return fail(kUnsupported, "w4 (tcgen05): %d work items exceed one launch", items);
     const int na = mode == 1 ? 2 : 1, ng = kStageK / w.group;
@@ -607,7 +594,7 @@ int launch_w4_umma(int mode, int wt, const W4KernelParams& kp, const W4Weights& 
     if (!map_tokens(&mx, kp.X, x_rows, kp.k, wt, np)) return fail(kUnsupported, "w4 (tcgen05): activation tensor map rejected");
     const size_t tile = kRaw + 256 * ng + (zp ? 128 * ng : 0);
     const size_t rings = (size_t)token_stages(np) * np * 256 + (size_t)raw_stages(na) * na * tile;
-    const size_t partial = sk > 1 ? (size_t)na * std::min(np, 64) * kTileM * 4 : 0;
+    const size_t partial = sk > 1 ? (size_t)std::min(np, 64) * kTileM * 4 : 0;
     const size_t smem = prepare_kernel(kern, kThreads, std::max(rings, partial) + 1024, tmem_columns(na, np));
     if (smem == 0) return fail(kCudaError, "w4 (tcgen05): a CTA with %d tokens does not fit on this device", np);
     int static_weights = option(kOptStaticWeights);
