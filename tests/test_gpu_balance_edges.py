@@ -1,4 +1,5 @@
-"""Balance loss at the ends of its range."""
+"""Balance loss at the ends of its range: strongly negative logits under sigmoid scores, derivatives of other kinds,
+counts in a captured graph."""
 import pytest
 import torch
 
@@ -106,6 +107,25 @@ def test_second_order_of_the_rest(T):
     assert torch.allclose(w.grad, 36 * w.detach() ** 3, rtol=1e-5) and x.grad is None
     with pytest.raises(RuntimeError, match="once"):
         gx.sum().backward()
+
+
+@pytest.mark.parametrize("masked", [False, True])
+def test_expert_counts_in_a_graph(masked):
+    """Captured without a call before it, replayed with other picks: every replay starts from zero."""
+    require_gpu()
+    g = torch.Generator().manual_seed(1)
+    draws = [torch.randint(-1, 20, (700, 3), generator=g, dtype=torch.int32) for _ in range(3)]
+    mask = (torch.rand(700, generator=g) < 0.5).cuda() if masked else None
+    ids = draws[0].cuda()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        counts = mlk().expert_counts(ids, 16, mask)
+    for d in draws + draws[:1]:
+        ids.copy_(d)
+        graph.replay()
+        rows = d if mask is None else d[mask.cpu()]
+        want = torch.bincount(rows[(rows >= 0) & (rows < 16)].long(), minlength=16)
+        assert torch.equal(counts.cpu().long(), want)
 
 
 def test_oracle_used_here_holds_far_from_zero():
