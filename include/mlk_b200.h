@@ -349,18 +349,19 @@ int mlk_layoutA_w4(const void* src, void* dst, int64_t m, int k, int inverse, ml
 /* elem_bytes: 2 (scales) or 1 (zero points). */
 int mlk_layoutA_w4_groups(const void* src, void* dst, int64_t m, int groups, int elem_bytes, mlk_stream_t s);
 /* C[n,m] = alpha * B[n,k] * W^T (+ bias), any n >= 0, m and k up to 2^28; dtype 0 / 1 = bf16 / fp16 scales, B, C and bias.
- * zeros may be NULL (8 everywhere); of each zero point the low four bits count.  Sums in fp32, rounded once.  Up to 16 tokens
- * the weights' value is exact; larger calls multiply the value rounded to the activation type.  status: sticky error word
- * of the bounded waits, or NULL. */
+ * zeros may be NULL (8 everywhere); of each zero point the low four bits count.  Sums in fp32, rounded once.  Up to 16
+ * tokens the weights' value is exact; larger calls multiply the value rounded to the activation type (a caller who needs the
+ * exact value passes 16 tokens at a time).  status: sticky error word of the bounded waits, or NULL. */
 int mlk_gemm_layoutA_w4(const void* A, const void* scales, const void* zeros, int group, const void* B, void* C, int m, int n,
                         int k, int dtype, float alpha, const void* bias, int32_t* status, mlk_stream_t s);
 /* Expert compute with 4-bit weights: y[t] = sum_j topk_weights[t,j] * W2_e (silu(Wgate_e x_t) * (Wup_e x_t)), e =
  * topk_ids[t,j] (through experts_map if given; ids without an expert here are skipped).  w1 [expert_count, 2 inter, hidden]
  * (gate rows, then up rows) and w2 [expert_count, hidden, inter] packed, with their own group sizes; hidden and inter
- * multiples of 32 and whole groups; at most 1024 experts and 8257408 slots (batch_size * topK).  Up to 4 routed slots per expert on average the weights' value is exact, above that it
- * is rounded to the activation type, as the activation between the two products always is.  y [T, hidden] in the activation type, or fp32 un-rounded sums with out_fp32 != 0;
- * every element of y is written.  workspace: mlk_experts_w4_workspace_bytes(...) bytes, 16-byte aligned, contents
- * irrelevant, not shared by calls that can overlap on the GPU. */
+ * multiples of 32 and whole groups; at most 1024 experts and 8257408 slots (batch_size * topK).  Up to 4 slots per expert of
+ * w1 (slots without an expert here included) the weights' value is exact, above that it is rounded to the activation type,
+ * as the activation between the two products always is.  y [T, hidden] in the activation type, or fp32 un-rounded sums with
+ * out_fp32 != 0; every element of y is written.  workspace: mlk_experts_w4_workspace_bytes(...) bytes, 16-byte aligned,
+ * contents irrelevant, not shared by calls that can overlap on the GPU. */
 int64_t mlk_experts_w4_workspace_bytes(int batch_size, int expert_count, int topK, int hidden, int inter);
 int mlk_fused_experts_compute_w4(const void* w1, const void* w1_scales, const void* w1_zeros, int w1_group, const void* w2,
                                  const void* w2_scales, const void* w2_zeros, int w2_group, const void* x, int batch_size,

@@ -250,11 +250,12 @@ def fused_moe_w4(
     out_dtype: Optional[torch.dtype] = None,
     out: Optional[torch.Tensor] = None,
     return_routing: bool = False,
+    exact_weights: bool = False,
 ):
     """The layer of ``fused_moe`` with expert weights in 4 bits and group scales: router (with the renormalisation of the
     top-k weights), then ``fused_experts_compute_w4``.  Same routing arguments; no host synchronisation, capturable in a
-    CUDA graph.  ``return_routing=True`` gives ``(y, topk_ids, topk_weights)``, for ``expert_counts`` (load statistics of a
-    server) or ``router_balance_loss``.  The reference has no counterpart."""
+    CUDA graph.  ``exact_weights``: as in ``fused_experts_compute_w4``.  ``return_routing=True`` gives ``(y, topk_ids,
+    topk_weights)``, for ``expert_counts`` (load statistics of a server) or ``router_balance_loss``.  The reference has no counterpart."""
     assert gate_weight is not None or hidden_states.shape[0] == gating_output.shape[0], "Number of tokens mismatch"
     if w1_scale is None or w2_scale is None:
         raise ValueError("4-bit weights need their group scales")
@@ -278,7 +279,7 @@ def fused_moe_w4(
         experts_map = experts_map.to(torch.int)
     with _Range("planC.experts"):
         y = fused_experts_compute_w4(w1, w1_scale, w2, w2_scale, hidden_states, topk_ids, topk_weights, w1_zeros, w2_zeros,
-                                     experts_map, out, out_dtype)
+                                     experts_map, out, out_dtype, exact_weights)
     return (y, topk_ids, topk_weights) if return_routing else y
 
 

@@ -27,6 +27,7 @@ __all__ = ["layoutA_w4", "layoutA_w4_inverse", "layoutA_w4_groups", "gemv_layout
            "fused_experts_compute_w4"]
 
 _GROUPS = (32, 64, 128)
+_EXACT_TOKENS, _EXACT_SLOTS = 16, 4     # tokens of a product, slots per expert, up to which the kernels do not round the weights
 _LIMIT = 2 ** 31        # the C interface's sizes are 32-bit integers, and ctypes cuts off what is longer
 _CODES = {torch.bfloat16: 0, torch.float16: 1}
 _device_of_thread = torch._C._cuda_getDevice
@@ -58,6 +59,11 @@ def _same_device(like: torch.Tensor, *named) -> None:
 
 def _fits(*sizes) -> None:
     _chk(max(sizes) < _LIMIT, "sizes of 2^31 and more are not supported")
+
+
+def _parts(n: int, step: int):
+    """(first row, rows) of the launches that take n rows in order, at most `step` at a time."""
+    return [(i, min(step, n - i)) for i in range(0, n, step)]
 
 
 def layoutA_w4(W: torch.Tensor) -> torch.Tensor:
@@ -140,11 +146,13 @@ def _group(A, scales, zeros, x, k: int, name: str) -> int:
     raise RuntimeError(f"{name}: weights, scales and zeros do not belong together")
 
 
-def gemm_layoutA_w4(A, scales, B, alpha: float = 1, beta: float = 0, zeros=None, bias=None):
+def gemm_layoutA_w4(A, scales, B, alpha: float = 1, beta: float = 0, zeros=None, bias=None, exact_weights: bool = False):
     """``C[n,m] = alpha * B W^T (+ bias)`` for any token count n (0 included), W in 4 bits: ``A`` from ``layoutA_w4``,
     ``scales`` / ``zeros`` from ``layoutA_w4_groups``, ``B[n,k]`` and C row-major.  Sums are held in fp32 and rounded once.
     ``beta`` is ignored, as by the other GEMMs.  Up to 16 tokens the weights' value is exact; larger calls multiply
-    the value rounded to the activation type (what a dequantised checkpoint holds)."""
+    the value rounded to the activation type (what a dequantised checkpoint holds), so that a token's result may differ
+    with the number of tokens in the call.  ``exact_weights=True`` keeps the value exact for any n, by launches of 16
+    tokens, each of which reads the weights."""
     _chk(B.is_cuda, "B must be a CUDA tensor")
     _chk(B.is_contiguous(), "B must be contiguous")
     _chk(B.dim() == 2, "B must be a 2D tensor")
@@ -161,8 +169,9 @@ def gemm_layoutA_w4(A, scales, B, alpha: float = 1, beta: float = 0, zeros=None,
         bias = _bias_ptr(bias, B, m)
     C = B.new_empty((n, m))
     d = B.get_device()
-    _launch(d, lib.mlk_gemm_layoutA_w4, A.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(), group,
-            B.data_ptr(), C.data_ptr(), m, n, k, code, alpha, bias, _status(d, B))
+    for i, count in _parts(n, _EXACT_TOKENS) if exact_weights else ((0, n),):
+        _launch(d, lib.mlk_gemm_layoutA_w4, A.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(), group,
+                B.data_ptr() + 2 * i * k, C.data_ptr() + 2 * i * m, m, count, k, code, alpha, bias, _status(d, B))
     return C
 
 
@@ -174,15 +183,18 @@ def gemv_layoutA_w4(A, scales, B, alpha: float = 1, beta: float = 0, zeros=None,
 
 def fused_experts_compute_w4(w1, w1_scales, w2, w2_scales, activations, topk_ids, topk_weights, w1_zeros=None, w2_zeros=None,
                              experts_map=None, out: Optional[torch.Tensor] = None,
-                             out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+                             out_dtype: Optional[torch.dtype] = None, exact_weights: bool = False) -> torch.Tensor:
     """``y[t] = sum_j topk_weights[t,j] * W2_e (silu(Wgate_e x_t) * (Wup_e x_t))``, ``e = topk_ids[t,j]``, expert weights in
     4 bits: ``w1 [E, 2I/16, ceil(H/64), 32, 16]`` (gate rows, then up rows) and ``w2 [E, H/16, ceil(I/64), 32, 16]`` from
     ``layoutA_w4``, scales and zero points from ``layoutA_w4_groups``; ``activations [T, H]`` bf16 / fp16, ``topk_ids``
     int32 ``[T, topk]``, ``topk_weights`` in the activations' type.  ``experts_map``: global -> local expert or -1, as in
     ``fused_experts_compute``; ids without an expert here contribute nothing.  ``out_dtype=torch.float32`` gives the
     un-rounded sums; ``out`` receives the result (every element is written).  A token's experts are added in
-    slot order in fp32 with one rounding.  At most 1024 experts and 8257408 slots (T * topk).  Up to 4 routed slots per expert on average the weights' value is exact; above
-    that it is rounded to the activation type, as the activation between the two products always is."""
+    slot order in fp32 with one rounding.  At most 1024 experts and 8257408 slots (T * topk).  Up to 4 slots (T * topk,
+    those without an expert here included) per expert of ``w1`` the weights' value is exact; above that it is rounded to
+    the activation type, as the activation between the two products always is, so that a token's result may differ with
+    the number of tokens in the call.  ``exact_weights=True`` keeps the value exact for any T, by launches of as many
+    tokens as that allows, each of which reads the weights of the experts that they pick."""
     x = activations
     _chk(x.is_cuda and x.is_contiguous(), "activations must be a contiguous CUDA tensor")
     _chk(x.dim() == 2, "activations must be [T, H]")
@@ -215,10 +227,18 @@ def fused_experts_compute_w4(w1, w1_scales, w2, w2_scales, activations, topk_ids
     else:
         _chk(out.get_device() == d and out.is_contiguous() and out.shape == x.shape and out.dtype is dtype,
              "out must be a contiguous [T, H] in the result's data type on the activations' device")
-    nbytes = lib.mlk_experts_w4_workspace_bytes(T, E, topk, H, I)
+    parts, most = ((0, T),), T
+    if exact_weights:
+        # a single token of up to 8 picks takes a path of its own, which does not round either
+        _chk(topk <= max(_EXACT_SLOTS * E, 8), f"exact_weights: {topk} picks of {E} experts are more than {_EXACT_SLOTS} per expert")
+        most = max(_EXACT_SLOTS * E // topk, 1)
+        parts = _parts(T, most)
+    nbytes = lib.mlk_experts_w4_workspace_bytes(min(T, most), E, topk, H, I)
     ws = x.new_empty((nbytes,), dtype=torch.uint8)
-    _launch(d, lib.mlk_fused_experts_compute_w4, w1.data_ptr(), w1_scales.data_ptr(), _ptr(w1_zeros), g1, w2.data_ptr(),
-            w2_scales.data_ptr(), _ptr(w2_zeros), g2, x.data_ptr(), T, E, topk, H, I, topk_ids.data_ptr(),
-            topk_weights.data_ptr(), out.data_ptr(), code, int(dtype is torch.float32), mp, ml, ws.data_ptr(), nbytes,
-            _status(d, x))
+    for i, count in parts:
+        _launch(d, lib.mlk_fused_experts_compute_w4, w1.data_ptr(), w1_scales.data_ptr(), _ptr(w1_zeros), g1, w2.data_ptr(),
+                w2_scales.data_ptr(), _ptr(w2_zeros), g2, x.data_ptr() + 2 * i * H, count, E, topk, H, I,
+                topk_ids.data_ptr() + 4 * i * topk, topk_weights.data_ptr() + 2 * i * topk,
+                out.data_ptr() + out.element_size() * i * H, code, int(dtype is torch.float32), mp, ml, ws.data_ptr(), nbytes,
+                _status(d, x))
     return out

@@ -187,3 +187,69 @@ def test_largest_number_of_slots():
         mlk().fused_experts_compute_w4(a[0], a[1], b[0], b[1], one_more, torch.zeros(T + 1, topk, dtype=torch.int32, device=dev),
                                        torch.zeros(T + 1, topk, dtype=torch.bfloat16, device=dev), w2_zeros=b[2])
     assert mlk().kernel_status() == 0
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("n", [0, 1, 16, 17, 32, 45, 130])
+def test_products_with_exact_weights_of_any_token_count(n, dtype):
+    """The weights of the test above: the rounded product lies outside the bound of the exact one, as the default shows."""
+    dev = require_gpu()
+    m, k, dt = 48, 160, DT[dtype]
+    off, d, s = worst_rounded(dt)
+    w = (torch.full((m, k), 8 + d, dtype=torch.uint8), torch.full((m, k // 32), s / 64, dtype=dt), None)
+    A, S, _ = laid_out(w, dev)
+    x, b = torch.ones(n, k, dtype=dt), randn((m,), 2, 1.0, dt)
+    x[:, 1:] = randn((n, k - 1), 3, 1.0, dt).abs()
+    want, bound = ow4.dense(*w, 32, x, alpha=0.5, bias=b)
+    got = mlk().gemm_layoutA_w4(A, S, x.to(dev), alpha=0.5, bias=b.to(dev), exact_weights=True)
+    check(got, want, bound, (n, dtype))
+    plain = mlk().gemm_layoutA_w4(A, S, x.to(dev), alpha=0.5, bias=b.to(dev))
+    if n <= 16:
+        assert torch.equal(got, plain)
+    else:
+        # the same bits whatever shares the call, 16 tokens at a time
+        assert torch.equal(got[16:32], mlk().gemm_layoutA_w4(A, S, x[16:32].to(dev), alpha=0.5, bias=b.to(dev)))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("case", [(2, 2, 1), (2, 2, 40), (8, 2, 50), (2, 5, 9), (3, 8, 4), (1, 1, 300)])
+def test_experts_with_exact_weights_of_any_token_count(case, dtype):
+    dev = require_gpu()
+    E, topk, T = case
+    H, I, dt = 128, 64, DT[dtype]
+    off, d, s = worst_rounded(dt)
+    full = lambda m, k, scale: (torch.full((E, m, k), 8 + d, dtype=torch.uint8),  # noqa: E731
+                                torch.full((E, m, k // 32), s * scale, dtype=dt), None)
+    w1, w2 = full(2 * I, H, 2.0 ** -6), full(H, I, 2.0 ** -6)
+    a, b = laid_out(w1, dev), laid_out(w2, dev)
+    x = torch.ones(T, H, dtype=dt) * (1 + torch.arange(T).remainder(3).to(dt).unsqueeze(1) / 4)
+    ids = torch.randint(0, E + 1, (T, topk), generator=torch.Generator().manual_seed(1), dtype=torch.int32)
+    p = torch.ones(T, topk, dtype=dt)
+    args = [t.to(dev) for t in (x, ids, p)]
+    for f32 in (False, True):
+        want, bound = ow4.experts(w1, w2, 32, 32, x, ids, p, out_fp32=f32)
+        out = torch.full((T, H), float("nan"), dtype=torch.float32 if f32 else dt, device=dev)
+        got = mlk().fused_experts_compute_w4(a[0], a[1], b[0], b[1], *args, out=out, exact_weights=True,
+                                             out_dtype=torch.float32 if f32 else None)
+        assert got is out
+        check(got, want, bound + 1e-30, (case, dtype, f32))
+    if T * topk > 4 * E and T > 1:      # the default rounds here, and the bound tells
+        rough = mlk().fused_experts_compute_w4(a[0], a[1], b[0], b[1], *args, out_dtype=torch.float32)
+        assert ((rough.cpu().double() - want).abs() > bound).any()
+
+
+def test_exact_weights_refusals_and_layer():
+    dev = require_gpu()
+    from muxi_native_layout_kernels_b200.muxi_moe_planC import fused_moe_w4
+    E, topk, H, I, T = 4, 2, 64, 32, 30
+    w1, w2 = ow4.random_weights(2 * I, H, 32, torch.bfloat16, 1, True, (E,)), ow4.random_weights(H, I, 32, torch.bfloat16, 2, False, (E,))
+    a, b = laid_out(w1, dev), laid_out(w2, dev)
+    x, logits = randn((T, H), 3, 1.0, torch.bfloat16).to(dev), randn((T, E), 4, 1.0, torch.bfloat16).to(dev)
+    y, ids, p = fused_moe_w4(x, a[0], b[0], logits, topk, True, w1_scale=a[1], w2_scale=b[1], w1_zeros=a[2], exact_weights=True,
+                             return_routing=True)
+    want, bound = ow4.experts(w1, w2, 32, 32, x.cpu(), ids.cpu(), p.cpu())
+    check(y, want, bound, "layer")
+    assert fused_moe_w4(x[:0], a[0], b[0], logits[:0], topk, True, w1_scale=a[1], w2_scale=b[1], exact_weights=True).shape == (0, H)
+    many = torch.zeros(2, 17, dtype=torch.int32, device=dev)
+    with pytest.raises(RuntimeError, match="exact_weights"):
+        mlk().fused_experts_compute_w4(a[0], a[1], b[0], b[1], x[:2], many, many.to(torch.bfloat16), exact_weights=True)
