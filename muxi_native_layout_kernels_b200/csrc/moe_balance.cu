@@ -147,17 +147,31 @@ __device__ __forceinline__ void scores(const Params& p, float (&x)[N], float (&o
     } else {
         // sigmoid(x) = e^min(x,0) / (1 + e^-|x|), taken here over e^m, m the row's largest min(x,0): the factor cancels in p, no
         // term overflows and the sum is at least 1/2, where the sigmoids themselves end below about -88 - ln E.  With a
-        // logit of 0 or more in the row m is 0.
-        float m = fminf(x[0], 0.f);
-#pragma unroll
-        for (int i = 1; i < N; ++i) m = fmaxf(m, fminf(x[i], 0.f));
-        m = group_max(m, p.lpr);
-        if (m == -INFINITY) m = 0.f;
+        // logit of 0 or more in the row m is 0 and one exponential does: a warp whose rows all have one, or nothing but -inf,
+        // skips the maximum and the second exponential (16384 x 128: 31 us the three kernels, with them in every row 33).
+        bool high = false, some = false;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const float e = expf(-fabsf(x[i])), d = 1.f / (1.f + e);
+            high |= x[i] >= 0.f;
+            some |= x[i] > -INFINITY;
+        }
+        const uint32_t row = (0xFFFFFFFFu >> (32 - p.lpr)) << (threadIdx.x & 31 & ~(p.lpr - 1));
+        const uint32_t highs = __ballot_sync(0xFFFFFFFFu, high) & row, somes = __ballot_sync(0xFFFFFFFFu, some) & row;
+        float m = 0.f;
+        if (!__all_sync(0xFFFFFFFFu, highs != 0u || somes == 0u)) {
+            m = fminf(x[0], 0.f);
+#pragma unroll
+            for (int i = 1; i < N; ++i) m = fmaxf(m, fminf(x[i], 0.f));
+            m = group_max(m, p.lpr);
+            if (m == -INFINITY) m = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float lo = fminf(x[i], 0.f), e = expf(-fabsf(x[i])), d = 1.f / (1.f + e);
             if constexpr (GRAD) one_minus[i] = x[i] >= 0.f ? e * d : d;
-            s += x[i] = expf(fminf(x[i], 0.f) - m) * d;          // NaN stays NaN through d
+            float f = x[i] >= 0.f ? 1.f : e;
+            if (m != 0.f) f = expf(lo - m);
+            s += x[i] = f * d;                                   // NaN stays NaN through d
         }
     }
     s = group_sum(s, p.lpr);
