@@ -38,7 +38,8 @@ struct W4Weights {
 //         sums (kFactorLow, kFactorHigh).  Two rows' pairs cost two ANDs and half a shift this way, where placing all four nibbles
 //         at the same position takes three shifts.
 //   fp16  The nibble is or-ed under the exponent of 1024: 1024 + q (low) or 1024 + 16 q (high); one packed fused
-//         multiply-add turns that into q - z, exact.
+//         multiply-add turns that into q - z, exact.  (The method of Kim, Henry, Fahim and Awadalla, "Who Says Elephants Can't
+//         Run: Bringing Large Scale MoE Models into Cloud Scale Production", 2022.)
 // `zl`, `zh`: the packed subtrahends of rows r and r + 8, made by zero() from a pair of zero-point bytes of which the low
 // four bits count.
 template <int WT>

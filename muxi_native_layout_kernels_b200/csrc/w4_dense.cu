@@ -28,9 +28,12 @@ int launch_w4_dense(const W4DenseParams& p, cudaStream_t s) {
     g.X = p.X;
     g.C = p.C;
     g.n = p.n;
-    // Up to 16 tokens the streaming kernel, which also keeps the weights exact, above it tcgen05.  Measured on both sides:
-    // 28672 x 8192 at 8 tokens 30 us against 36 (the tcgen05 kernel's decode and hand-offs cost the same for any token
-    // count), 4096 x 14336 at 16 tokens 17.5 against 15.5, 14336 x 4096 at 61 tokens 65 against 16.8.
+    // Up to 16 tokens the streaming kernel, above it tcgen05, whose decode and hand-offs cost the same for any token count.
+    // By time the border would be near 8: 28672 x 8192 at 8 tokens 30 us against 36; from 9 tokens on (9 / 12 / 16 tokens)
+    // 46 / 48 / 51 against 36.5, 4096 x 14336 17.0 / 17.2 / 17.6 against 15.7, 14336 x 4096 17.9 / 18.9 / 20.3 against 16.1,
+    // 8192 x 8192 15.5 / 15.7 / 16.7 against 16.2, 4096 x 4096 7.3 / 7.4 / 7.7 against 7.3, 1040 x 2080 5.5 / 5.5 / 5.9 against
+    // 4.9.  It stays at 16 because the streaming kernel keeps the weights exact, which a decode batch of that size is
+    // promised.  14336 x 4096 at 61 tokens: 65 against 16.8.
     if (p.n <= 16) return launch_w4_mma(0, p.dtype, g, p.w, 1, 1, p.n <= 8 ? 1 : 2, s);
     const W4UmmaPlan q = w4_umma_plan(g.out_tiles, p.n, p.k);
     const int tokens = (p.n + q.np - 1) / q.np;

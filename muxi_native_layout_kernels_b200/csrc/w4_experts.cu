@@ -140,7 +140,8 @@ int launch_w4_experts(const W4ExpertsParams& p, cudaStream_t s) {
         return launch_w4_mma(2, p.dtype, g, p.w2, p.topk, p.topk, 1, s);
     }
 
-    // Slots of a work item, by the slots an expert gets: the streaming kernel up to 4, above it tcgen05 with 32, 64 or 128.
+    // Slots of a work item, by the slots an expert gets (all routed slots over the experts here: with an experts_map the slots
+    // of other ranks count too, since only the device knows them): the streaming kernel up to 4, above it tcgen05 with 32, 64 or 128.
     // Measured (us): 2 slots 63 against 81, 4 slots 82 / 174 against 98 / 176, 8 slots 130 / 230 against 109 / 186 (128 experts of
     // 2048 x 768 / 8 of 4096 x 14336); 32 against 64 slots a tile: 127 / 190 against 142 / 215 at 16 slots, 173 / 273
     // against 170 / 231 at 32; 128 slots a tile: 497 against 542 at 128.
@@ -167,7 +168,9 @@ int launch_w4_experts(const W4ExpertsParams& p, cudaStream_t s) {
     if (np > 0) {
         // consecutive row tiles of a CTA of the second product: up to four where k is short and two rounds of two CTAs per SM
         // are left (128 experts of 2048 x 768, us with 1 / 2 / 4 / 8: 113 / 107 / 106 / 106 at 128 tokens, 152 / 144 / 141 / 141
-        // at 512; with k = 14336 it only costs, 193 / 220 / 303; nor does it pay for the first product)
+        // at 512; 60 of 2048 x 1408 at 512 tokens 119 / 116 / 116).  Where k is longer it costs: 16 experts, 256 tokens, us with 1 / 2
+        // / 4: 49 / 54 / 71 at 2048 x 2048 (the second bound keeps it at 1 there), 111 / 110 / 123 at 4096 x 2816, 90 / 96 / 122 at
+        // 2048 x 4096; 8 of 4096 x 8192 155 / 166 / 213, of 4096 x 14336 193 / 220 / 303.  Nor does it pay for the first product
         const int run = p.I > 2048 ? 1 : std::max(1, std::min(4, (int)((p.H + 127) / 128 * (long long)likely / (4LL * sm_count()))));
         // the token rows of a work item have to be contiguous for the tile copy; the gathered rows borrow the scratch
         if (int st = launch_gather(p.x, sorted, worklist, p.topk, p.H, scratch, slots, s)) return st;

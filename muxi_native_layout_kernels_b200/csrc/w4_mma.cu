@@ -8,9 +8,9 @@
 // multiplies the fp32 sums of a group, not the weights.  Measured on the arithmetic alone (operands from shared memory, no
 // other traffic): 16.8 T weights/s with one column tile of 8 tokens, 11 T with two; HBM delivers 13 T; a copy of the
 // weights into shared memory alone takes 21 us for the 117 MB of 28672 x 8192, with the arithmetic 25.
-// Measured (us, and of the time that the bytes take at the copy bandwidth): 4096 x 4096 at 1 token 5.6 (1.3: one wave of
-// CTAs, latency), 28672 x 8192 at 8 tokens 31 (18.6), 4096 x 14336 fp16 with zero points at 16 tokens 17 (5.0), 8 of 128 experts of 2048 x 768 for one token 14.4 (3.0: two kernels of latency), 33
-// tokens on them 63 (42), 5 tokens on 8 experts of 4096 x 14336 118 (85).  At 28672 x 8192 and 8 tokens a word takes 16
+// Measured (us, and of the time that the bytes take at the copy bandwidth): 4096 x 4096 at 1 token 5.8 (1.3: one wave of
+// CTAs, latency), 28672 x 8192 at 8 tokens 31 (18.6), 4096 x 14336 fp16 with zero points at 16 tokens 17.5 (5.0), 8 of 128 experts of 2048 x 768 for one token 15.3 (3.0: two
+// kernels of latency), 33 tokens on them 63 (42), 5 tokens on 8 experts of 4096 x 14336 123 (85).  At 28672 x 8192 and 8 tokens a word takes 16
 // warp instructions in all, and the issue slots are 54 % busy, the ALU pipe 45 %, the tensor pipe 27 %: the warps wait for
 // one another's pipes, not for memory.  More than 16 tokens go to the tcgen05 kernel.
 //

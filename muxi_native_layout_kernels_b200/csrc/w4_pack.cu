@@ -1,6 +1,8 @@
 // Prepack of 4-bit weights (format in w4.cuh): row-major nibbles <-> 512-byte blocks, and the pair order of scales and
 // zero points.  Run once per matrix at load time; a thread moves one lane's 16 bytes of a block (eight 2-byte reads, one
-// 16-byte store), bound by HBM.
+// 16-byte store).  What bounds it: the 2-byte accesses to the row-major side.  28672 x 8192 (117 MB in, 117 MB out; 36 us at the
+// copy bandwidth) takes 60 us, the way back, with 2-byte stores, 118 us; the scales of that matrix in groups of 32 (29 MB in all,
+// 4.5 us) 21 us.  Not made faster: 100 GB of packed weights take 50 ms, once.
 #include "w4.cuh"
 
 namespace mlk {

@@ -15,8 +15,8 @@
 // between the roles, at NP = 256 the tensor pipe.  Small grids split k over a cluster; partial tiles are added through
 // distributed shared memory in a fixed order.
 // Measured (us, and the floor by bytes or by the tensor peak): 14336 x 4096 with zero points per 32 at 61 tokens 17.2 (5.7;
-// issue slots 49 % busy, tensor pipe 27 %), 8192 x 8192 at 500 tokens 54 at full clocks, 62 under the power cap (40.6; tensor pipe
-// 62 %), 512 tokens x 8 on 128 experts of 2048 x 768 in fp16 with zero points 153, under the power cap 168 (51).
+// issue slots 49 % busy, tensor pipe 27 %), 8192 x 8192 at 500 tokens 53 at full clocks, 62 under the power cap (40.6; tensor pipe
+// 62 %), 512 tokens x 8 on 128 experts of 2048 x 768 in fp16 with zero points 151, under the power cap 165-173 (51).
 // The parts of a stage overlap only in part: at 37888 x 8192 and 64 tokens (45 us) a copy without the stores to tensor memory
 // took 41, without the MMAs 36, without the decode 38, with none of them 30.  An MMA with its rows in tensor memory takes
 // 20 / 32 / 64 / 128 cycles at 32 / 64 / 128 / 256 tokens.  Three slots, six raw stages, or one CTA per SM with all of the
