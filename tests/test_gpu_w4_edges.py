@@ -253,3 +253,42 @@ def test_exact_weights_refusals_and_layer():
     many = torch.zeros(2, 17, dtype=torch.int32, device=dev)
     with pytest.raises(RuntimeError, match="exact_weights"):
         mlk().fused_experts_compute_w4(a[0], a[1], b[0], b[1], x[:2], many, many.to(torch.bfloat16), exact_weights=True)
+
+
+@pytest.mark.parametrize("static", [False, True])
+def test_exact_weights_in_parts_share_their_workspace_in_order(static):
+    """The launches of one call follow one another closely, over one workspace: the same bits eager, captured and replayed, and
+    with the weights fetched ahead."""
+    dev = require_gpu()
+    E, topk, H, I, T = 4, 2, 256, 96, 150
+    w = laid_out(ow4.random_weights(H, H, 128, torch.bfloat16, 5, True), dev)
+    a = laid_out(ow4.random_weights(2 * I, H, 128, torch.bfloat16, 1, False, (E,)), dev)
+    b = laid_out(ow4.random_weights(H, I, 32, torch.bfloat16, 2, True, (E,)), dev)
+    x = randn((T, H), 3, 1.0, torch.bfloat16).to(dev)
+    ids = torch.rand(T, E, generator=torch.Generator().manual_seed(6)).topk(topk, -1)[1].to(torch.int32).to(dev)
+    p = torch.full((T, topk), 0.5, dtype=torch.bfloat16, device=dev)
+
+    def chain():
+        y = mlk().fused_experts_compute_w4(a[0], a[1], b[0], b[1], x, ids, p, w2_zeros=b[2], exact_weights=True)
+        return mlk().gemm_layoutA_w4(w[0], w[1], y, alpha=0.25, zeros=w[2], exact_weights=True)
+
+    alone = []
+    for i in range(0, T, 8):        # the parts one at a time, each with a workspace of its own
+        rows = slice(i, i + 8)
+        alone.append(mlk().fused_experts_compute_w4(a[0], a[1], b[0], b[1], x[rows].contiguous(), ids[rows].contiguous(),
+                                                    p[rows].contiguous(), w2_zeros=b[2]))
+        torch.cuda.synchronize()
+    y = torch.cat(alone)
+    want = torch.cat([mlk().gemm_layoutA_w4(w[0], w[1], y[i:i + 16].contiguous(), alpha=0.25, zeros=w[2]) for i in range(0, T, 16)])
+    torch.cuda.synchronize()
+    mlk().set_static_weights(static)
+    try:
+        assert torch.equal(chain(), want)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = chain()
+        for _ in range(5):
+            graph.replay()
+        assert torch.equal(got, want) and mlk().kernel_status() == 0
+    finally:
+        mlk().set_static_weights(False)
